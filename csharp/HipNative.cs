@@ -155,6 +155,13 @@ internal static unsafe class HipNative
                                                                  int axis, LxTensor* y);
     [DllImport(Lib)] public static extern int lx_ElementwiseChain(LxTensor** inputs, int nIn, int* ops, int* operands,
                                                                   int nOps, LxTensor* y);
+    [DllImport(Lib)] public static extern int lx_QuantizeBlocks(LxTensor* x, long to, long blockRows, LxTensor* q,
+                                                                LxTensor* scales);
+    [DllImport(Lib)] public static extern int lx_MatMulBlocks(LxTensor* a, LxTensor* aScale, LxTensor* b, LxTensor* bScale,
+                                                              LxTensor* bias, LxTensor* y);
+    [DllImport(Lib)] public static extern int lx_TokenLogProbs(LxTensor* logits, LxTensor* ids, long top,
+                                                               LxTensor* logProbs, LxTensor* entropy, LxTensor* topIds,
+                                                               LxTensor* topLogProbs);
 
     // ---- diagnostics ---------------------------------------------------------------------------
     [DllImport(Lib)] public static extern int lx_read_probe(IntPtr src, long bytes, IntPtr output, long outBytes);

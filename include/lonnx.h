@@ -30,7 +30,10 @@ extern "C" {
 enum lx_dtype {
     LX_FLOAT = 1, LX_UINT8 = 2, LX_INT8 = 3, LX_UINT16 = 4, LX_INT16 = 5,
     LX_INT32 = 6, LX_INT64 = 7, LX_BOOL = 9, LX_DOUBLE = 11, LX_UINT32 = 12,
-    LX_UINT64 = 13
+    LX_UINT64 = 13,
+    /* 8-bit floating point codes (the numbers of ONNX's TensorProto.DataType; not in the reference): taken by
+     * lx_QuantizeBlocks and lx_MatMulBlocks alone. */
+    LX_FLOAT8E4M3FN = 17, LX_FLOAT8E5M2 = 19
 };
 
 /* Status codes returned by every entry point (0 = success). */
@@ -231,6 +234,34 @@ enum { LX_CHAIN_ADD = 0, LX_CHAIN_SUB = 1, LX_CHAIN_MUL = 2, LX_CHAIN_DIV = 3, L
        LX_CHAIN_SQRT = 16, LX_CHAIN_ERF = 17 };
 int lx_ElementwiseChain(const lx_tensor *const *inputs, int32_t n_in, const int32_t *ops, const int32_t *operands,
                         int32_t n_ops, lx_tensor *Y);
+
+/* ---- scoring: 8-bit products and token log-probabilities (no reference counterpart) ------------------
+ * What a program runs behind a model's last hidden states: weights and activations as 8-bit floating point
+ * codes with a Float scale for each block of 128 values (4x less to read than Float), their product, and
+ * what the logits say about tokens.  Outputs that the caller provides must not overlap the inputs or each
+ * other (LX_ERR_INVALID_ARGUMENT); nothing is read back, so every one of them can be captured. */
+/* Codes Q (type `to`: LX_FLOAT8E4M3FN or LX_FLOAT8E5M2, X's shape) and scales of X (Float, rank >= 1): one
+ * scale for every 128 neighbours of the last axis (block_rows 1: scales [..., ceil(K / 128)] for X [..., K]) or
+ * for every 128 x 128 block of the last two axes (block_rows 128: [..., ceil(N / 128), ceil(K / 128)]); the last
+ * block of an axis may be smaller.  scale = amax / MAX (448; 57344), amax the largest finite magnitude of the
+ * block, at least 2^-126, and 1 for a block without a finite nonzero value; code = the nearest to x / scale of
+ * the exact quotient, ties to even.  Infinities saturate to +-MAX, NaN stays NaN. */
+int lx_QuantizeBlocks(const lx_tensor *X, int64_t to, int64_t block_rows, lx_tensor *Q, lx_tensor *scales);
+/* Y[..., m, n] = sum over blocks j of K of a_scale[..., m, j] * b_scale[n', j] * (sum over k in block j of
+ * A[..., m, k] * B[n, k]), plus bias[n] when bias is not NULL.  A [..., M, K] (or [K]) and B [N, K] are 8-bit
+ * codes of either type, each its own; B is stored as [N, K] (a weight matrix by output channel).  a_scale is
+ * [..., M, ceil(K / 128)]; b_scale is [ceil(N / 128), ceil(K / 128)] (n' = n / 128) or [N, ceil(K / 128)]
+ * (n' = n).  Y is Float; sums are Float, products exact.  A row of A that holds NaN gives a row of NaN. */
+int lx_MatMulBlocks(const lx_tensor *A, const lx_tensor *a_scale, const lx_tensor *B, const lx_tensor *b_scale,
+                    const lx_tensor *bias, lx_tensor *Y);
+/* For each row of logits [..., V] (Float): log_probs [...] = log softmax(logits)[ids], for ids [...] (Int32 or
+ * Int64; a negative id marks a row without a token: 0; an id of V or more: NaN), entropy [...] of the row's
+ * distribution in nats, and the `top` (0..64) most probable ids and their log-probabilities, [..., top], most
+ * probable first, equal logits by index (NaN logits last).  ids and log_probs are given together or both NULL,
+ * top_ids and top_log_probs exactly when top > 0, entropy may be NULL; at least one output is asked for.
+ * A logit of -inf has probability 0; a row whose logits are all -inf, or that holds NaN or +inf, gives NaN. */
+int lx_TokenLogProbs(const lx_tensor *logits, const lx_tensor *ids, int64_t top, lx_tensor *log_probs,
+                     lx_tensor *entropy, lx_tensor *top_ids, lx_tensor *top_log_probs);
 
 /* ---- operator profiling: the OpStage.Math stage of eager calls ------------------
  * The reference's operators open profiler stages as they go (Profiler.StartOpStage, Profiler.cs:71-80;

@@ -10,6 +10,7 @@ MAX_RANK = 8
 
 # TensorElementType codes (Tensor.cs:31-50)
 FLOAT, UINT8, INT8, UINT16, INT16, INT32, INT64, BOOL, DOUBLE, UINT32, UINT64 = 1, 2, 3, 4, 5, 6, 7, 9, 11, 12, 13
+FLOAT8E4M3FN, FLOAT8E5M2 = 17, 19
 
 # lx_status
 OK = 0
@@ -127,6 +128,9 @@ SIGNATURES = {
     "lx_MatMulAddGelu": (_c.c_int, [_T, _T, _T, _T]),
     "lx_ScaleAddSoftmax": (_c.c_int, [_T, _T, _c.c_int32, _T, _c.c_int32, _T]),
     "lx_ElementwiseChain": (_c.c_int, [_c.POINTER(_T), _c.c_int32, _i32p, _i32p, _c.c_int32, _T]),
+    "lx_QuantizeBlocks": (_c.c_int, [_T, _c.c_int64, _c.c_int64, _T, _T]),
+    "lx_MatMulBlocks": (_c.c_int, [_T, _T, _T, _T, _T, _T]),
+    "lx_TokenLogProbs": (_c.c_int, [_T, _T, _c.c_int64, _T, _T, _T, _T]),
     "lx_read_probe": (_c.c_int, [_c.c_void_p, _c.c_int64, _c.c_void_p, _c.c_int64]),
     "lx_pool_trim": (_c.c_int, []),
     "lx_pool_stats": (_c.c_int, [_i64p, _i64p]),

@@ -107,7 +107,7 @@ int64_t esize(int dt) {
     switch (dt) {
     case LX_FLOAT: case LX_INT32: case LX_UINT32: return 4;
     case LX_DOUBLE: case LX_INT64: case LX_UINT64: return 8;
-    case LX_UINT8: case LX_INT8: case LX_BOOL: return 1;
+    case LX_UINT8: case LX_INT8: case LX_BOOL: case LX_FLOAT8E4M3FN: case LX_FLOAT8E5M2: return 1;
     case LX_UINT16: case LX_INT16: return 2;
     default: return 0;
     }
@@ -119,9 +119,14 @@ const char *dtype_name(int dt) {
     case 5: return "Int16"; case 6: return "Int32"; case 7: return "Int64"; case 8: return "String";
     case 9: return "Bool"; case 10: return "Float16"; case 11: return "Double"; case 12: return "UInt32";
     case 13: return "UInt64"; case 14: return "Complex64"; case 15: return "Complex128"; case 16: return "BFloat16";
+    case 17: return "Float8E4M3FN"; case 19: return "Float8E5M2";
     default: return "Unknown";
     }
 }
+
+// The 8-bit floating types exist for QuantizeBlocks and MatMulBlocks alone: every other operator and the graph
+// runtime work on the reference's element types.
+bool is_f8(int dt) { return dt == LX_FLOAT8E4M3FN || dt == LX_FLOAT8E5M2; }
 
 std::string lower(std::string s) {
     for (auto &c : s) c = (char)tolower(c);
@@ -864,7 +869,7 @@ int api_set_error(int code, const std::string &message) {
 }
 bool api_initialized() { return g.init; }
 hipStream_t api_stream() { return g.stream; }
-int64_t api_esize(int dtype) { return esize(dtype); }
+int64_t api_esize(int dtype) { return is_f8(dtype) ? 0 : esize(dtype); }
 const char *api_dtype_name(int dtype) { return dtype_name(dtype); }
 void api_defer_checks(ErrFlags *slot, DeferredCheck *rec) {
     t_defer_slot = slot;
@@ -1189,10 +1194,10 @@ int lx_Cast(const lx_tensor *X, int64_t to, lx_tensor *Y) {
     int st;
     if ((st = check_tensor(X, "input"))) return st;
     const int dst = (int)to;
-    if (to != dst || !esize(dst))  // Float16 / BFloat16 / Complex / String targets (CPUExecutionProvider.cs:470-473)
+    if (to != dst || !esize(dst) || is_f8(dst))  // Float16 / BFloat16 / Complex / String targets (CPUExecutionProvider.cs:470-473)
         return set_err(LX_ERR_ATTRIBUTE_NOT_SUPPORTED,
                        "The attribute to with value %lld is not supported for operation Cast. ", (long long)to);
-    if (!esize(X->dtype))
+    if (!esize(X->dtype) || is_f8(X->dtype))
         return set_err(LX_ERR_INPUT_TYPE_NOT_SUPPORTED, "Object must implement IConvertible.");
     if ((st = prepare_output(Y, dst, X->rank, X->dims))) return st;
     const int64_t n = numel(X);
@@ -2188,7 +2193,7 @@ extern "C" int lx_MatMulAddGelu(const lx_tensor *A, const lx_tensor *B, const lx
 // ===========================================================================
 namespace {
 
-bool movable_dtype(int dt) { return esize(dt) != 0; }
+bool movable_dtype(int dt) { return esize(dt) != 0 && !is_f8(dt); }
 
 int64_t row_major_strides(int rank, const int64_t *dims, int64_t *str) {
     int64_t s = 1;
@@ -2423,6 +2428,7 @@ extern "C" int lx_Slice(const lx_tensor *data, const int64_t *starts, int32_t n_
     if (!ends || n_ends < 0) return missing_input("Slice", "ends");
     int st;
     if ((st = check_tensor(data, "data"))) return st;
+    if (is_f8(data->dtype)) return not_supported("Slice");
     // CPUExecutionProvider.Slice checks (CPUExecutionProvider.cs:554-560); the rank-1 checks of the
     // starts / ends / axes / steps tensors are made by the caller that holds them as tensors
     auto shape_err = [&](const char *param, const std::string &shape, const char *msg) {
@@ -2497,4 +2503,248 @@ extern "C" int lx_Slice(const lx_tensor *data, const int64_t *starts, int32_t n_
         a.src_base += sstart[d] * in_str[d];
     }
     return view_copy(data->dtype, data->data, Y->data, a);
+}
+
+// ===========================================================================
+// The scoring operators (no reference counterpart): block-scaled 8-bit
+// floating point products and the log-probabilities of tokens.
+// ===========================================================================
+namespace {
+
+int wrong_shape(const char *name, const lx_tensor *t, const std::string &want) {
+    return set_err(LX_ERR_WRONG_INPUT_SHAPE, "The input tensor  for parameter %s has shape %s but is required to have shape %s.",
+                   name, print_shape(t).c_str(), want.c_str());
+}
+
+std::string shape_text(int rank, const int64_t *dims) {
+    lx_tensor t{};
+    t.rank = rank;
+    for (int i = 0; i < rank; i++) t.dims[i] = dims[i];
+    return print_shape(&t);
+}
+
+bool has_shape(const lx_tensor *t, int rank, const int64_t *dims) {
+    if (t->rank != rank) return false;
+    for (int i = 0; i < rank; i++)
+        if (t->dims[i] != dims[i]) return false;
+    return true;
+}
+
+// A tensor the kernels read by elements: its address a multiple of the element size.
+int check_element_alignment(const lx_tensor *t, const char *name) {
+    if ((uintptr_t)t->data % esize(t->dtype))
+        return set_err(LX_ERR_INVALID_ARGUMENT, "The storage of tensor %s is not aligned to its elements.", name);
+    return LX_OK;
+}
+
+// The output must not share storage with an input: its blocks are written while others are still to be read.
+int check_apart(const lx_tensor *out, const char *oname, const lx_tensor *in, const char *iname) {
+    if (overlaps(out->data, numel(out) * esize(out->dtype), in->data, numel(in) * esize(in->dtype)))
+        return set_err(LX_ERR_INVALID_ARGUMENT, "The output %s shares storage with %s.", oname, iname);
+    return LX_OK;
+}
+
+int64_t blocks128(int64_t n) { return (n + 127) / 128; }
+
+// Outputs this call allocated go back to the pool when it fails after all.
+struct OutputGuard {
+    lx_tensor *t;
+    bool given, keep = false;
+    explicit OutputGuard(lx_tensor *y) : t(y), given(!y || y->data) {}
+    ~OutputGuard() {
+        if (!keep && !given) (void)lx_tensor_free(t);
+    }
+};
+
+}  // namespace
+
+extern "C" int lx_QuantizeBlocks(const lx_tensor *X, int64_t to, int64_t block_rows, lx_tensor *Q, lx_tensor *scales) {
+    OpScope prof("QuantizeBlocks");
+    REQUIRE_INIT();
+    if (!X) return missing_input("QuantizeBlocks", "X");
+    int st;
+    if ((st = check_tensor(X, "X"))) return st;
+    if (X->dtype != LX_FLOAT) return type_not_supported("QuantizeBlocks", "X", X);
+    if (to != LX_FLOAT8E4M3FN && to != LX_FLOAT8E5M2)
+        return set_err(LX_ERR_ATTRIBUTE_NOT_SUPPORTED,
+                       "The attribute to with value %lld is not supported for operation QuantizeBlocks. ", (long long)to);
+    if (block_rows != 1 && block_rows != 128)
+        return set_err(LX_ERR_ATTRIBUTE_NOT_SUPPORTED,
+                       "The attribute block_rows with value %lld is not supported for operation QuantizeBlocks. ",
+                       (long long)block_rows);
+    if (X->rank < (block_rows == 1 ? 1 : 2))
+        return set_err(LX_ERR_WRONG_INPUT_SHAPE, "The input tensor  for parameter X has shape %s but is required to have rank %d.",
+                       print_shape(X).c_str(), block_rows == 1 ? 1 : 2);
+    if ((st = check_element_alignment(X, "X"))) return st;
+    int64_t sd[LX_MAX_RANK];
+    for (int i = 0; i < X->rank; i++) sd[i] = X->dims[i];
+    const int64_t k = X->dims[X->rank - 1];
+    sd[X->rank - 1] = blocks128(k);
+    int64_t mats = 1, rows = 1;
+    for (int i = 0; i < X->rank - 1; i++) (block_rows == 1 || i == X->rank - 2 ? rows : mats) *= X->dims[i];
+    if (block_rows == 128) sd[X->rank - 2] = blocks128(rows);
+    if (!Q || !scales || Q == scales) return set_err(LX_ERR_INVALID_ARGUMENT, "The output tensor handle is null.");
+    OutputGuard gq(Q), gs(scales);
+    if ((st = prepare_output(Q, (int)to, X->rank, X->dims)) || (st = prepare_output(scales, LX_FLOAT, X->rank, sd))) return st;
+    if ((st = check_element_alignment(scales, "scales")) || (st = check_apart(Q, "Q", X, "X")) ||
+        (st = check_apart(scales, "scales", X, "X")) || (st = check_apart(scales, "scales", Q, "Q")))
+        return st;
+    if (numel(X)) {
+        const QuantizeArgs a = {(const float *)X->data, (uint8_t *)Q->data, (float *)scales->data, mats, rows, k,
+                                (int32_t)block_rows, (int32_t)to};
+        HIPCHECK(launch_quantize_blocks(a, g.stream), "QuantizeBlocks");
+    }
+    gq.keep = gs.keep = true;
+    return LX_OK;
+}
+
+extern "C" int lx_MatMulBlocks(const lx_tensor *A, const lx_tensor *a_scale, const lx_tensor *B, const lx_tensor *b_scale,
+                               const lx_tensor *bias, lx_tensor *Y) {
+    OpScope prof("MatMulBlocks");
+    REQUIRE_INIT();
+    if (!A) return missing_input("MatMulBlocks", "A");
+    if (!a_scale) return missing_input("MatMulBlocks", "a_scale");
+    if (!B) return missing_input("MatMulBlocks", "B");
+    if (!b_scale) return missing_input("MatMulBlocks", "b_scale");
+    int st;
+    if ((st = check_tensor(A, "A")) || (st = check_tensor(a_scale, "a_scale")) || (st = check_tensor(B, "B")) ||
+        (st = check_tensor(b_scale, "b_scale")) || (bias && (st = check_tensor(bias, "bias"))))
+        return st;
+    if (!is_f8(A->dtype)) return type_not_supported("MatMulBlocks", "A", A);
+    if (!is_f8(B->dtype)) return type_not_supported("MatMulBlocks", "B", B);
+    if (a_scale->dtype != LX_FLOAT) return type_not_supported("MatMulBlocks", "a_scale", a_scale);
+    if (b_scale->dtype != LX_FLOAT) return type_not_supported("MatMulBlocks", "b_scale", b_scale);
+    if (bias && bias->dtype != LX_FLOAT) return type_not_supported("MatMulBlocks", "bias", bias);
+    if (A->rank < 1)
+        return set_err(LX_ERR_WRONG_INPUT_SHAPE, "The input tensor  for parameter A has shape %s but is required to have rank %d.",
+                       print_shape(A).c_str(), 1);
+    if (B->rank != 2)
+        return set_err(LX_ERR_WRONG_INPUT_SHAPE, "The input tensor  for parameter B has shape %s but is required to have rank %d.",
+                       print_shape(B).c_str(), 2);
+    const int64_t k = A->dims[A->rank - 1], n = B->dims[0];
+    if (B->dims[1] != k)
+        return set_err(LX_ERR_INVALID_ARGUMENT,
+                       "The number of columns in the first matrix (%lld) is not equal to the number of columns in the second "
+                       "matrix (%lld).",
+                       (long long)k, (long long)B->dims[1]);
+    int64_t od[LX_MAX_RANK], sd[LX_MAX_RANK], m = 1;
+    for (int i = 0; i < A->rank; i++) sd[i] = od[i] = A->dims[i];
+    for (int i = 0; i < A->rank - 1; i++) m *= A->dims[i];
+    sd[A->rank - 1] = blocks128(k);
+    od[A->rank - 1] = n;
+    if (!has_shape(a_scale, A->rank, sd)) return wrong_shape("a_scale", a_scale, shape_text(A->rank, sd));
+    const int64_t by_row[2] = {n, blocks128(k)}, by_block[2] = {blocks128(n), blocks128(k)};
+    const bool rows = has_shape(b_scale, 2, by_row);
+    if (!rows && !has_shape(b_scale, 2, by_block))
+        return wrong_shape("b_scale", b_scale, shape_text(2, by_block) + " or " + shape_text(2, by_row));
+    if (bias && !has_shape(bias, 1, &n)) return wrong_shape("bias", bias, shape_text(1, &n));
+    if (m > INT32_MAX || n > INT32_MAX || k > INT32_MAX)
+        return set_err(LX_ERR_NOT_SUPPORTED, "Matrix dimensions beyond 2^31 are not supported.");
+    if ((st = check_element_alignment(a_scale, "a_scale")) || (st = check_element_alignment(b_scale, "b_scale")) ||
+        (bias && (st = check_element_alignment(bias, "bias"))))
+        return st;
+    if (!Y) return set_err(LX_ERR_INVALID_ARGUMENT, "The output tensor handle is null.");
+    OutputGuard gy(Y);
+    if ((st = prepare_output(Y, LX_FLOAT, A->rank, od))) return st;
+    if ((st = check_element_alignment(Y, "Y")) || (st = check_apart(Y, "Y", A, "A")) || (st = check_apart(Y, "Y", B, "B")) ||
+        (st = check_apart(Y, "Y", a_scale, "a_scale")) || (st = check_apart(Y, "Y", b_scale, "b_scale")) ||
+        (bias && (st = check_apart(Y, "Y", bias, "bias"))))
+        return st;
+    if (m && n) {
+        MatMulBlocksArgs p;
+        memset(&p, 0, sizeof p);
+        p.a = (const uint8_t *)A->data;
+        p.b = (const uint8_t *)B->data;
+        p.sa = (const float *)a_scale->data;
+        p.sb = (const float *)b_scale->data;
+        p.bias = bias ? (const float *)bias->data : nullptr;
+        p.y = (float *)Y->data;
+        p.m = m;
+        p.n = n;
+        p.k = k;
+        p.fmt_a = A->dtype;
+        p.fmt_b = B->dtype;
+        p.b_rows = rows ? 1 : 128;
+        HIPCHECK(launch_matmul_blocks(p, g.stream), "MatMulBlocks");
+    }
+    gy.keep = true;
+    return LX_OK;
+}
+
+extern "C" int lx_TokenLogProbs(const lx_tensor *logits, const lx_tensor *ids, int64_t top, lx_tensor *log_probs,
+                                lx_tensor *entropy, lx_tensor *top_ids, lx_tensor *top_log_probs) {
+    OpScope prof("TokenLogProbs");
+    REQUIRE_INIT();
+    if (!logits) return missing_input("TokenLogProbs", "logits");
+    int st;
+    if ((st = check_tensor(logits, "logits")) || (ids && (st = check_tensor(ids, "ids")))) return st;
+    if (logits->dtype != LX_FLOAT) return type_not_supported("TokenLogProbs", "logits", logits);
+    if (ids && ids->dtype != LX_INT32 && ids->dtype != LX_INT64) return type_not_supported("TokenLogProbs", "ids", ids);
+    if (logits->rank < 1)
+        return set_err(LX_ERR_WRONG_INPUT_SHAPE,
+                       "The input tensor  for parameter logits has shape %s but is required to have rank %d.",
+                       print_shape(logits).c_str(), 1);
+    const int rank = logits->rank - 1;
+    const int64_t v = logits->dims[rank];
+    if (ids && !has_shape(ids, rank, logits->dims)) return wrong_shape("ids", ids, shape_text(rank, logits->dims));
+    if (v < 1 || v > INT32_MAX - 64)
+        return set_err(LX_ERR_NOT_SUPPORTED, "A vocabulary of %lld tokens is not supported.", (long long)v);
+    if (top < 0 || top > kLogProbsTop || top > v)
+        return set_err(LX_ERR_ATTRIBUTE_NOT_SUPPORTED,
+                       "The attribute top with value %lld is not supported for operation TokenLogProbs. ", (long long)top);
+    if (!ids != !log_probs)
+        return set_err(LX_ERR_INVALID_ARGUMENT, "Log-probabilities and the token ids they are for must be given together.");
+    if (!top != !top_ids || !top != !top_log_probs)
+        return set_err(LX_ERR_INVALID_ARGUMENT, "The most probable ids, their log-probabilities and their number must be "
+                                                "given together.");
+    if (!log_probs && !entropy && !top) return set_err(LX_ERR_INVALID_ARGUMENT, "The output tensor handle is null.");
+    if (rank + (top ? 1 : 0) > LX_MAX_RANK) return set_err(LX_ERR_NOT_SUPPORTED, "At most %d axes are supported.", LX_MAX_RANK);
+    if ((st = check_element_alignment(logits, "logits")) || (ids && (st = check_element_alignment(ids, "ids")))) return st;
+    struct Out {
+        lx_tensor *t;
+        const char *name;
+        int dtype;
+        bool wide;
+    } outs[4] = {{log_probs, "log_probs", LX_FLOAT, false}, {entropy, "entropy", LX_FLOAT, false},
+                 {top_ids, "top_ids", LX_INT64, true}, {top_log_probs, "top_log_probs", LX_FLOAT, true}};
+    int64_t od[LX_MAX_RANK], t = 1;
+    for (int i = 0; i < rank; i++) t *= od[i] = logits->dims[i];
+    if (top) od[rank] = top;
+    OutputGuard guards[4] = {OutputGuard(log_probs), OutputGuard(entropy), OutputGuard(top_ids), OutputGuard(top_log_probs)};
+    for (int i = 0; i < 4; i++) {
+        if (!outs[i].t) continue;
+        for (int j = 0; j < i; j++)
+            if (outs[j].t == outs[i].t) return set_err(LX_ERR_INVALID_ARGUMENT, "Two outputs share one tensor handle.");
+        if ((st = prepare_output(outs[i].t, outs[i].dtype, rank + outs[i].wide, od)) ||
+            (st = check_element_alignment(outs[i].t, outs[i].name)) ||
+            (st = check_apart(outs[i].t, outs[i].name, logits, "logits")) ||
+            (ids && (st = check_apart(outs[i].t, outs[i].name, ids, "ids"))))
+            return st;
+        for (int j = 0; j < i; j++)
+            if (outs[j].t && (st = check_apart(outs[i].t, outs[i].name, outs[j].t, outs[j].name))) return st;
+    }
+    if (t) {
+        LogProbsArgs a;
+        memset(&a, 0, sizeof a);
+        a.x = (const float *)logits->data;
+        a.ids = ids ? ids->data : nullptr;
+        a.ids_dtype = ids ? ids->dtype : 0;
+        a.lp = log_probs ? (float *)log_probs->data : nullptr;
+        a.h = entropy ? (float *)entropy->data : nullptr;
+        a.top_ids = top ? (int64_t *)top_ids->data : nullptr;
+        a.top_lp = top ? (float *)top_log_probs->data : nullptr;
+        a.t = t;
+        a.v = v;
+        a.top = (int32_t)top;
+        hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
+        (void)hipStreamIsCapturing(g.stream, &cs);
+        const bool capturing = cs != hipStreamCaptureStatusNone;
+        const int64_t bytes = logprobs_part_bytes(a);
+        if (bytes) HIPCHECK(alloc_temp(&a.part, bytes, capturing), "device allocation (temporary)");
+        const hipError_t e = launch_logprobs(a, g.stream);
+        release_temp(a.part, capturing);
+        if (e != hipSuccess) return hip_fail(e, "TokenLogProbs");
+    }
+    for (auto &k : guards) k.keep = true;
+    return LX_OK;
 }

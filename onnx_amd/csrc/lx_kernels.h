@@ -13,7 +13,7 @@ namespace lx {
 // TensorElementType codes (Tensor.cs:31-50)
 enum DType : int {
     kFloat = 1, kUInt8 = 2, kInt8 = 3, kUInt16 = 4, kInt16 = 5, kInt32 = 6, kInt64 = 7,
-    kBool = 9, kDouble = 11, kUInt32 = 12, kUInt64 = 13
+    kBool = 9, kDouble = 11, kUInt32 = 12, kUInt64 = 13, kFloat8E4M3FN = 17, kFloat8E5M2 = 19
 };
 
 enum BinOp : int { kAdd = 0, kSub = 1, kMul = 2, kDiv = 3, kPow = 4 };
@@ -230,6 +230,44 @@ hipError_t launch_matmul(int dtype, const void *a, const void *b, void *c, const
 bool matmul_ln_fusable(int dtype, const void *a, const void *b, const void *c, const MatMulArgs &p);
 hipError_t launch_matmul_ln(const void *a, const void *b, void *y, const MatMulArgs &p, const float *gamma,
                             const float *beta, float eps, hipStream_t s);
+
+// QuantizeBlocks: mats matrices of [rows, k] floats to 8-bit codes of fmt with a scale for each block of block_rows
+// (1 or 128) rows by 128 columns, scales row-major over [mats, blocks of rows, blocks of columns].  k > 0.
+struct QuantizeArgs {
+    const float *x;
+    uint8_t *q;
+    float *s;
+    int64_t mats, rows, k;
+    int32_t block_rows, fmt;
+};
+hipError_t launch_quantize_blocks(const QuantizeArgs &a, hipStream_t s);
+
+// MatMulBlocks: y[m, n] = a[m, k] b[n, k]^T of 8-bit codes (fmt_a, fmt_b) with scales sa [m, ceil(k / 128)] and sb
+// [n or ceil(n / 128), ceil(k / 128)] (b_rows 1 or 128), plus bias[n] unless null.  m, n > 0 and below 2^31.
+struct MatMulBlocksArgs {
+    const uint8_t *a, *b;
+    const float *sa, *sb, *bias;
+    float *y;
+    int64_t m, n, k;
+    int32_t fmt_a, fmt_b, b_rows;
+};
+hipError_t launch_matmul_blocks(const MatMulBlocksArgs &p, hipStream_t s);
+
+// TokenLogProbs over t rows of v logits (v > 0): the log-probability of ids[row] (Int32 / Int64; null: none), the
+// entropy (null: not asked) and the `top` most probable ids with theirs (top 0: none).  part: logprobs_part_bytes
+// of scratch.
+constexpr int kLogProbsTop = 64;
+struct LogProbsArgs {
+    const float *x;
+    const void *ids;
+    float *lp, *h, *top_lp;
+    int64_t *top_ids;
+    int64_t t, v;
+    int32_t ids_dtype, top;
+    void *part;
+};
+int64_t logprobs_part_bytes(const LogProbsArgs &a);
+hipError_t launch_logprobs(const LogProbsArgs &a, hipStream_t s);
 
 // Data movement (Transpose, Slice, Concat, expand): for every index j of `dims`
 //   dst[dst_base + sum_k j_k dst_str[k]] = src[src_base + sum_k j_k src_str[k]]

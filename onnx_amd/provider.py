@@ -20,6 +20,14 @@ NP_OF = {L.FLOAT: np.float32, L.UINT8: np.uint8, L.INT8: np.int8, L.UINT16: np.u
          L.INT32: np.int32, L.INT64: np.int64, L.BOOL: np.bool_, L.DOUBLE: np.float64, L.UINT32: np.uint32,
          L.UINT64: np.uint64}
 CODE_OF = {np.dtype(v): k for k, v in NP_OF.items()}
+# 8-bit floating point codes: numpy has no such types, so the host sees their bytes
+F8_OF = {L.FLOAT8E4M3FN: np.uint8, L.FLOAT8E5M2: np.uint8}
+
+
+def _code(dtype):
+    """The element type code of a numpy dtype, or the code of an 8-bit floating type itself."""
+    return dtype if isinstance(dtype, int) and dtype in F8_OF else CODE_OF[np.dtype(dtype)]
+
 
 _initialised = False
 
@@ -60,15 +68,18 @@ class DeviceTensor:
     def empty(cls, shape, dtype):
         init()
         h = L.LxTensor()
-        code = CODE_OF[np.dtype(dtype)]
+        code = _code(dtype)
         _check(L.lib().lx_tensor_alloc(code, len(shape), L.dims_array(shape), ctypes.byref(h)), "lx_tensor_alloc")
         return cls(h)
 
     @classmethod
-    def from_numpy(cls, arr):
+    def from_numpy(cls, arr, element_type=None):
+        """Uploads arr.  element_type: FLOAT8E4M3FN or FLOAT8E5M2 for an array of bytes that are such codes."""
         arr = np.asarray(arr)
         arr = np.ascontiguousarray(arr).reshape(arr.shape)  # keeps rank 0
-        t = cls.empty(arr.shape, arr.dtype)
+        if element_type is not None and (element_type not in F8_OF or arr.dtype != np.uint8):
+            raise TypeError(f"element type {element_type} of {arr.dtype} values")
+        t = cls.empty(arr.shape, arr.dtype if element_type is None else element_type)
         _check(L.lib().lx_tensor_upload(ctypes.byref(t.h), ctypes.c_void_p(arr.ctypes.data), arr.nbytes),
                "lx_tensor_upload")
         return t
@@ -85,7 +96,7 @@ class DeviceTensor:
         """Non-owning view of existing device memory (e.g. a torch tensor)."""
         init()
         h = L.LxTensor()
-        _check(L.lib().lx_tensor_wrap(CODE_OF[np.dtype(dtype)], len(shape), L.dims_array(shape),
+        _check(L.lib().lx_tensor_wrap(_code(dtype), len(shape), L.dims_array(shape),
                                       ctypes.c_void_p(ptr), capacity, ctypes.byref(h)), "lx_tensor_wrap")
         return cls(h, keepalive)
 
@@ -94,7 +105,8 @@ class DeviceTensor:
         import torch  # plumbing only: device memory comes from torch's allocator
         np_dtype = {torch.float32: np.float32, torch.float64: np.float64, torch.int32: np.int32,
                     torch.int64: np.int64, torch.uint8: np.uint8, torch.int8: np.int8, torch.int16: np.int16,
-                    torch.bool: np.bool_}[t.dtype]
+                    torch.bool: np.bool_, torch.float8_e4m3fn: L.FLOAT8E4M3FN,
+                    torch.float8_e5m2: L.FLOAT8E5M2}[t.dtype]
         assert t.is_contiguous()
         return cls.wrap(t.data_ptr(), tuple(t.shape), np_dtype, t.numel() * t.element_size(), keepalive=t)
 
@@ -105,7 +117,7 @@ class DeviceTensor:
 
     @property
     def dtype(self):
-        return np.dtype(NP_OF[self.h.dtype])
+        return np.dtype(F8_OF.get(self.h.dtype) or NP_OF[self.h.dtype])
 
     @property
     def ElementType(self):
@@ -431,3 +443,52 @@ class HipExecutionProvider:
         S, mask = _as_tensor(S), _as_tensor(mask)
         y = out.h if out is not None else L.LxTensor()
         return _result("AddSoftmax", L.lib().lx_AddSoftmax(_ptr(S), _ptr(mask), int(axis), ctypes.byref(y)), y, out)
+
+    # ---- scoring: 8-bit products and token log-probabilities -------------------
+    @staticmethod
+    def _results(op, st, handles, out):
+        """OpResult of an operator with several outputs; `out`: the caller's output tensors, one for each, or None."""
+        if st == L.OK:
+            return OpResult(op, OpStatus.Success, None, list(out) if out else [DeviceTensor(h) for h in handles], 0)
+        return OpResult(op, OpStatus.Failure, L.last_error(), [], st)
+
+    @staticmethod
+    def _outputs(n, out):
+        """The handles of n outputs: the caller's, or empty ones for the operator to allocate."""
+        if out is not None and len(out) != n:
+            raise ValueError(f"{len(out)} output tensors for {n} outputs")
+        return [t.h for t in out] if out is not None else [L.LxTensor() for _ in range(n)]
+
+    @staticmethod
+    def QuantizeBlocks(X, to=L.FLOAT8E4M3FN, block_rows=1, out=None):
+        """8-bit floating point codes of a Float tensor with one Float scale for each 1x128 (block_rows=1) or
+        128x128 (block_rows=128) block of the last axes: Outputs [codes, scales] (lx_QuantizeBlocks)."""
+        init()
+        X = _as_tensor(X)
+        q, s = HipExecutionProvider._outputs(2, out)
+        st = L.lib().lx_QuantizeBlocks(_ptr(X), int(to), int(block_rows), ctypes.byref(q), ctypes.byref(s))
+        return HipExecutionProvider._results("QuantizeBlocks", st, (q, s), out)
+
+    @staticmethod
+    def MatMulBlocks(A, a_scale, B, b_scale, bias=None, out=None):
+        """Product of two block-scaled 8-bit matrices, A [..., M, K] and B [N, K] (by output channel), plus a bias
+        row: Float [..., M, N] (lx_MatMulBlocks)."""
+        init()
+        A, a_scale, B, b_scale, bias = (_as_tensor(t) for t in (A, a_scale, B, b_scale, bias))
+        y = out.h if out is not None else L.LxTensor()
+        st = L.lib().lx_MatMulBlocks(_ptr(A), _ptr(a_scale), _ptr(B), _ptr(b_scale), _ptr(bias), ctypes.byref(y))
+        return _result("MatMulBlocks", st, y, out)
+
+    @staticmethod
+    def TokenLogProbs(logits, ids=None, top=0, entropy=False, out=None):
+        """Of each row of logits [..., V]: the log-probability of ids [...] (with ids), the entropy in nats (with
+        entropy) and the `top` most probable ids and their log-probabilities (with top): Outputs holds those asked
+        for, in that order (lx_TokenLogProbs)."""
+        init()
+        logits, ids = _as_tensor(logits), _as_tensor(ids)
+        asked = [ids is not None, bool(entropy), int(top) != 0, int(top) != 0]
+        given = HipExecutionProvider._outputs(sum(asked), out)
+        it = iter(given)
+        handles = [ctypes.byref(next(it)) if a else None for a in asked]
+        st = L.lib().lx_TokenLogProbs(_ptr(logits), _ptr(ids), int(top), *handles)
+        return HipExecutionProvider._results("TokenLogProbs", st, given, out)
