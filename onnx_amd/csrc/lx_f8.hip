@@ -266,11 +266,198 @@ __global__ __launch_bounds__(256) void k_matmul_blocks_small(MatMulBlocksArgs p)
     }
 }
 
-template <int FA, int FB> static hipError_t matmul_blocks(const MatMulBlocksArgs &p, hipStream_t s) {
-    const int64_t tiles = (p.m + 31) / 32 * ((p.n + 31) / 32);
-    if (p.b_rows == 1) k_matmul_blocks_small<FA, FB, true><<<(unsigned)tiles, 256, 0, s>>>(p);
-    else k_matmul_blocks_small<FA, FB, false><<<(unsigned)tiles, 256, 0, s>>>(p);
+// ---- tiles of Y through LDS -------------------------------------------------------------------------------------
+// A workgroup computes BM x BN of Y (BM = 32 TM WM rows, BN = 32 TN WN columns); each of its WM x WN waves TM x TN
+// tiles of 32x32.  A stage of LDS holds one block of K: BM rows of A and BN rows of B, 128 codes each, and their
+// scales; S stages are filled by direct-to-LDS loads S - 1 blocks ahead, with one barrier a block.  The codes stay 8
+// bits in LDS (half the traffic of bf16) and are converted as a wave reads them.  Row r's 16-byte chunk c lies at
+// slot c ^ ((r >> 1) & 7): the 32 rows a fragment read touches then spread over all banks.
+// Operands need rows of whole 16-byte chunks (k a multiple of 16, aligned storage) and tiles within 2^31 bytes.
+__device__ __forceinline__ uint32_t f8_lds(const void *p) {
+    return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char *)p;
+}
+// The lane's 16 (4) bytes at base + off land in LDS at lds + 16 (4) * lane; lds is uniform over the wave.  Inline asm
+// so that the compiler does not make LDS reads of other stages wait for them; the kernel waits itself.
+__device__ __forceinline__ void f8_load_lds16(const void *base, uint32_t off, void *lds) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    __asm__ volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"{m0}"(f8_lds(lds)), "v"(off), "s"(base) : "memory");
+#endif
+}
+__device__ __forceinline__ void f8_load_lds4(const void *base, uint32_t off, void *lds) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    __asm__ volatile("s_nop 0\n\tglobal_load_lds_dword %1, %2" ::"{m0}"(f8_lds(lds)), "v"(off), "s"(base) : "memory");
+#endif
+}
+// All but this wave's last N direct loads have landed and its LDS operations are done, then the workgroup's barrier.
+template <int N> __device__ __forceinline__ void f8_wait_barrier() {
+    static_assert(N >= 0 && N < 64, "vmcnt range");
+    __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4));
+#if defined(__HIP_DEVICE_COMPILE__)
+    __asm__ volatile("s_barrier" ::: "memory");
+#endif
+}
+
+template <int FA, int FB, bool BROWS, int TM, int TN, int WM, int WN, int S, int OCC>
+__global__ __launch_bounds__(64 * WM * WN, OCC) void k_matmul_blocks(MatMulBlocksArgs p, int tm, int tn) {
+    constexpr int NW = WM * WN, BM = 32 * TM * WM, BN = 32 * TN * WN, R = BM + BN;
+    constexpr int L = R / 8 / NW;               // 16-byte loads a wave and stage, of eight rows each
+    constexpr int LS = (R / 64 + NW - 1) / NW;  // 4-byte loads of the rows' scales
+    static_assert(R % (8 * NW) == 0 && R % 64 == 0 && BM % 8 == 0 && BN <= 128, "whole wave loads");
+    constexpr int STAGE = R * 128 + LS * NW * 256;
+    __shared__ __attribute__((aligned(1024))) char sm[S][STAGE];
+    const int l = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = l >> 5;
+
+    // tiles in groups of eight rows of tiles, contiguous ranges of them to each XCD (workgroups go round the 8 XCDs)
+    const int tiles = tm * tn, per = (tiles + 7) / 8;
+    const int t = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    if ((int)(blockIdx.x >> 3) >= per || t >= tiles) return;
+    const int group = t / (8 * tn), first = 8 * group, gs = min(tm - first, 8), in = t - group * 8 * tn;
+    const int m0 = (first + in % gs) * BM, n0 = in / gs * BN;
+
+    const int64_t kb = (p.k + 127) / 128;
+    const uint8_t *abase = p.a + m0 * p.k, *bbase = p.b + n0 * p.k;
+    const int row_n = BROWS ? 1 : 128;
+    const float *sabase = p.sa + m0 * kb, *sbbase = p.sb + n0 / row_n * kb;
+    uint32_t off[L], soff[LS];
+#pragma unroll
+    for (int i = 0; i < L; i++) {
+        const int r = 8 * (w + NW * i) + (l >> 3), c = (l & 7) ^ ((r >> 1) & 7);
+        const int row = r < BM ? min(r, (int)p.m - 1 - m0) : min(r - BM, (int)p.n - 1 - n0);
+        off[i] = (uint32_t)(row * (int)p.k + 16 * c);
+    }
+#pragma unroll
+    for (int i = 0; i < LS; i++) {
+        const int r = min(64 * (w + NW * i) + l, R - 1);
+        const int row = r < BM ? min(r, (int)p.m - 1 - m0) : min(r - BM, (int)p.n - 1 - n0) / row_n;
+        soff[i] = (uint32_t)(row * (int)kb * 4);
+    }
+    const int tail = (int)(p.k & 127);  // codes of a last block that is not whole
+    auto load = [&](int64_t j, char *st) {
+        const bool cut = tail && j == kb - 1;
+#pragma unroll
+        for (int i = 0; i < L; i++) {
+            const bool is_a = 8 * (w + NW * i) < BM;  // uniform: eight rows are all A's or all B's
+            const uint8_t *base = (is_a ? abase : bbase) + 128 * j;
+            char *lds = st + 1024 * (w + NW * i);
+            if (!cut) {
+                f8_load_lds16(base, off[i], lds);
+            } else {
+                const int r = 8 * (w + NW * i) + (l >> 3), c = (l & 7) ^ ((r >> 1) & 7);
+                if (16 * c < tail) f8_load_lds16(base, off[i], lds);
+                else *(uint4 *)(lds + 16 * l) = uint4{0, 0, 0, 0};
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < LS; i++) {
+            const bool is_a = 64 * (w + NW * i) < BM;
+            f8_load_lds4((is_a ? sabase : sbbase) + j, soff[i], st + R * 128 + 256 * (w + NW * i));
+        }
+    };
+
+    f8_v16f acc[TN][TM] = {};
+    const int wm = w % WM, wn = w / WM;
+    const int swz = ((l & 31) >> 1) & 7;
+    for (int s = 0; s < S - 1; s++)
+        if (s < kb) load(s, sm[s]);
+    int cur = 0;
+    for (int64_t j = 0; j < kb; j++) {
+        // the last S - 2 stages ahead may still be landing; near the end there are fewer
+        if (S > 2 && j + S - 2 < kb) f8_wait_barrier<(S - 2) * (L + LS)>();
+        else f8_wait_barrier<0>();
+        const char *st = sm[cur];
+        if (j + S - 1 < kb) load(j + S - 1, sm[cur == 0 ? S - 1 : cur - 1]);
+        cur = cur + 1 == S ? 0 : cur + 1;
+        const char *ap = st + (wm * TM * 32 + (l & 31)) * 128, *bp = st + (BM + wn * TN * 32 + (l & 31)) * 128;
+        f8_v16f part[TN][TM] = {};
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            uint4 va[TM], vb[TN];
+            const int slot = 16 * ((2 * c + h) ^ swz);
+#pragma unroll
+            for (int i = 0; i < TM; i++) va[i] = *(const uint4 *)(ap + i * 32 * 128 + slot);
+#pragma unroll
+            for (int i = 0; i < TN; i++) vb[i] = *(const uint4 *)(bp + i * 32 * 128 + slot);
+#pragma unroll
+            for (int z = 0; z < 2; z++) {
+                f8_v8bf a[TM], b[TN];
+#pragma unroll
+                for (int i = 0; i < TM; i++) a[i] = z ? f8_bf16x8<FA>(va[i].z, va[i].w) : f8_bf16x8<FA>(va[i].x, va[i].y);
+#pragma unroll
+                for (int i = 0; i < TN; i++) b[i] = z ? f8_bf16x8<FB>(vb[i].z, vb[i].w) : f8_bf16x8<FB>(vb[i].x, vb[i].y);
+#pragma unroll
+                for (int in_ = 0; in_ < TN; in_++)
+#pragma unroll
+                    for (int im = 0; im < TM; im++)
+                        part[in_][im] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(b[in_], a[im], part[in_][im], 0, 0, 0);
+            }
+        }
+        const float *sc = (const float *)(st + R * 128);
+        float sa[TM];
+#pragma unroll
+        for (int i = 0; i < TM; i++) sa[i] = sc[(wm * TM + i) * 32 + (l & 31)];
+#pragma unroll
+        for (int in_ = 0; in_ < TN; in_++) {
+            const float *sb = sc + BM + (wn * TN + in_) * 32 + 4 * h;
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                f8_v4f b4;
+                if constexpr (BROWS) b4 = *(const f8_v4f *)(sb + 8 * q);
+#pragma unroll
+                for (int im = 0; im < TM; im++) {
+                    const float one = sa[im] * sc[BM + wn * TN * 32];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const float f = BROWS ? sa[im] * b4[e] : one;
+                        acc[in_][im][4 * q + e] = __builtin_fmaf(part[in_][im][4 * q + e], f, acc[in_][im][4 * q + e]);
+                    }
+                }
+            }
+        }
+    }
+    const bool vec = p.n % 4 == 0 && ((uintptr_t)p.y & 15) == 0;
+#pragma unroll
+    for (int im = 0; im < TM; im++) {
+        const int64_t m = m0 + (wm * TM + im) * 32 + (l & 31);
+        if (m >= p.m) continue;
+#pragma unroll
+        for (int in_ = 0; in_ < TN; in_++)
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                const int64_t n = n0 + (wn * TN + in_) * 32 + 8 * q + 4 * h;
+                f8_v4f v;
+                for (int e = 0; e < 4; e++) v[e] = acc[in_][im][4 * q + e];
+                if (vec) {
+                    if (n < p.n) {
+                        if (p.bias)
+                            for (int e = 0; e < 4; e++) v[e] += p.bias[n + e];
+                        *(f8_v4f *)(p.y + m * p.n + n) = v;
+                    }
+                } else {
+                    for (int e = 0; e < 4; e++)
+                        if (n + e < p.n) p.y[m * p.n + n + e] = p.bias ? v[e] + p.bias[n + e] : v[e];
+                }
+            }
+    }
+}
+
+template <int FA, int FB, bool BROWS> static hipError_t matmul_blocks(const MatMulBlocksArgs &p, hipStream_t s) {
+    const bool chunks = p.k % 16 == 0 && p.k > 0 && (((uintptr_t)p.a | (uintptr_t)p.b) & 15) == 0 && p.k < (1 << 23);
+    const int64_t t128 = (p.m + 127) / 128 * ((p.n + 127) / 128), t64 = (p.m + 63) / 64 * ((p.n + 63) / 64);
+    if (chunks && t128 >= 256 && t128 < (1 << 26)) {
+        k_matmul_blocks<FA, FB, BROWS, 2, 2, 2, 2, 2, 2>
+            <<<(unsigned)((t128 + 7) / 8 * 8), 256, 0, s>>>(p, (int)((p.m + 127) / 128), (int)((p.n + 127) / 128));
+    } else if (chunks && p.m > 32 && t64 >= 256 && t64 < (1 << 26)) {
+        k_matmul_blocks<FA, FB, BROWS, 1, 1, 2, 2, 3, 3>
+            <<<(unsigned)((t64 + 7) / 8 * 8), 256, 0, s>>>(p, (int)((p.m + 63) / 64), (int)((p.n + 63) / 64));
+    } else {
+        const int64_t tiles = (p.m + 31) / 32 * ((p.n + 31) / 32);
+        k_matmul_blocks_small<FA, FB, BROWS><<<(unsigned)tiles, 256, 0, s>>>(p);
+    }
     return hipGetLastError();
+}
+
+template <int FA, int FB> static hipError_t matmul_blocks(const MatMulBlocksArgs &p, hipStream_t s) {
+    return p.b_rows == 1 ? matmul_blocks<FA, FB, true>(p, s) : matmul_blocks<FA, FB, false>(p, s);
 }
 
 hipError_t launch_matmul_blocks(const MatMulBlocksArgs &p, hipStream_t s) {
