@@ -2638,8 +2638,10 @@ extern "C" int lx_MatMulBlocks(const lx_tensor *A, const lx_tensor *a_scale, con
     if (!rows && !has_shape(b_scale, 2, by_block))
         return wrong_shape("b_scale", b_scale, shape_text(2, by_block) + " or " + shape_text(2, by_row));
     if (bias && !has_shape(bias, 1, &n)) return wrong_shape("bias", bias, shape_text(1, &n));
-    if (m > INT32_MAX || n > INT32_MAX || k > INT32_MAX)
+    if (m > INT32_MAX || n > INT32_MAX)
         return set_err(LX_ERR_NOT_SUPPORTED, "Matrix dimensions beyond 2^31 are not supported.");
+    if (k >= kMatMulBlocksK || (m + 31) / 32 * ((n + 31) / 32) > (1 << 23))
+        return set_err(LX_ERR_NOT_SUPPORTED, "Products over 2^23 columns and more, or of more than 2^23 tiles of 32x32, are not supported.");
     if ((st = check_element_alignment(a_scale, "a_scale")) || (st = check_element_alignment(b_scale, "b_scale")) ||
         (bias && (st = check_element_alignment(bias, "bias"))))
         return st;

@@ -212,58 +212,32 @@ template <int FMT> __device__ __forceinline__ f8_v8bf f8_bf16x8(unsigned lo, uns
     return r;
 }
 
-// 16 codes of a row from column c on, zeros (a code of value zero) past the row's end
-__device__ __forceinline__ uint4 f8_load16(const uint8_t *row, int64_t c, int64_t k) {
+// 16 codes of a row of k from column c on, as they lie in memory: the 16 that end with the row where fewer are left
+// (f8_tail16 moves them down), none from a column past it.  No byte outside the row is read.
+__device__ __forceinline__ uint4 f8_load16(const uint8_t *row, int c, int k) {
     uint4 v = {0, 0, 0, 0};
-    if (c + 16 <= k) {
-        __builtin_memcpy(&v, row + c, 16);
-    } else {
-        unsigned w[4] = {0, 0, 0, 0};
-#pragma unroll
-        for (int i = 0; i < 16; i++)
-            if (c + i < k) w[i / 4] |= (unsigned)row[c + i] << (8 * (i % 4));
-        v = {w[0], w[1], w[2], w[3]};
+    if (k < 16) {
+        uint64_t b[2] = {0, 0};
+        for (int i = c; i < k; i++) b[(i - c) / 8] |= (uint64_t)row[i] << (8 * ((i - c) & 7));
+        v = uint4{(unsigned)b[0], (unsigned)(b[0] >> 32), (unsigned)b[1], (unsigned)(b[1] >> 32)};
+    } else if (c < k) {
+        __builtin_memcpy(&v, row + min(c, k - 16), 16);
     }
     return v;
 }
-
-// One 32x32 tile of Y a workgroup, its four waves over every fourth block of K, their sums added in order.
-template <int FA, int FB, bool BROWS>
-__global__ __launch_bounds__(256) void k_matmul_blocks_small(MatMulBlocksArgs p) {
-    __shared__ f8_v16f part[3][64];
-    const int l = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = l >> 5;
-    const int64_t tiles_n = (p.n + 31) / 32;
-    const int64_t m0 = blockIdx.x / tiles_n * 32, n0 = blockIdx.x % tiles_n * 32;
-    const int64_t kb = (p.k + 127) / 128;
-    const int64_t m = std::min<int64_t>(m0 + (l & 31), p.m - 1), n = std::min<int64_t>(n0 + (l & 31), p.n - 1);
-    const uint8_t *ar = p.a + m * p.k, *br = p.b + n * p.k;
-    f8_v16f acc = {};
-    for (int64_t j = w; j < kb; j += 4) {
-        f8_v16f t = {};
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int64_t c = j * 128 + i * 32 + h * 16;
-            const uint4 va = f8_load16(ar, c, p.k), vb = f8_load16(br, c, p.k);
-            t = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f8_bf16x8<FB>(vb.x, vb.y), f8_bf16x8<FA>(va.x, va.y), t, 0, 0, 0);
-            t = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f8_bf16x8<FB>(vb.z, vb.w), f8_bf16x8<FA>(va.z, va.w), t, 0, 0, 0);
-        }
-        const float sa = p.sa[m * kb + j];
-#pragma unroll
-        for (int r = 0; r < 16; r++) {
-            const int64_t nr = std::min<int64_t>(n0 + 8 * (r / 4) + 4 * h + r % 4, p.n - 1);
-            const float sb = p.sb[(BROWS ? nr : nr / 128) * kb + j];
-            acc[r] = __builtin_fmaf(t[r], sa * sb, acc[r]);
-        }
+// what f8_load16 read for column c with the codes before c dropped and zeros (codes of value zero) past the row's end
+__device__ __forceinline__ uint4 f8_tail16(uint4 v, int c, int k) {
+    const int sh = c - (k - 16);
+    if (k < 16 || sh <= 0 || sh >= 16) return v;
+    uint64_t lo = v.x | (uint64_t)v.y << 32, hi = v.z | (uint64_t)v.w << 32;
+    if (sh >= 8) {
+        lo = hi;
+        hi = 0;
     }
-    if (w) part[w - 1][l] = acc;
-    __syncthreads();
-    if (w || m0 + (l & 31) >= p.m) return;
-    for (int i = 0; i < 3; i++) acc += part[i][l];
-#pragma unroll
-    for (int r = 0; r < 16; r++) {
-        const int64_t nr = n0 + 8 * (r / 4) + 4 * h + r % 4;
-        if (nr < p.n) p.y[m * p.n + nr] = p.bias ? acc[r] + p.bias[nr] : acc[r];
-    }
+    const int bits = 8 * (sh & 7);
+    if (bits) lo = lo >> bits | hi << (64 - bits);
+    hi >>= bits;
+    return uint4{(unsigned)lo, (unsigned)(lo >> 32), (unsigned)hi, (unsigned)(hi >> 32)};
 }
 
 // ---- tiles of Y through LDS -------------------------------------------------------------------------------------
@@ -297,14 +271,196 @@ template <int N> __device__ __forceinline__ void f8_wait_barrier() {
 #endif
 }
 
+// A block of K for a wave's TM x TN tiles of 32x32 is read in four chunks of 32 codes a row (the lane's 16 bytes of
+// chunk c are k = 32 c + 16 h .. + 15 of its row: the same permutation of k on both sides), and multiplied in eight
+// steps of half a chunk.
+template <int TM, int TN> struct F8Raw {
+    uint4 a[TM], b[TN];
+    // ap, bp: the lane's row of the wave's first tile of A's and of B's rows
+    __device__ __forceinline__ void read(const char *ap, const char *bp, int c, int h, int swz) {
+        const int slot = 16 * ((2 * c + h) ^ swz);
+#pragma unroll
+        for (int i = 0; i < TM; i++) a[i] = *(const uint4 *)(ap + i * 32 * 128 + slot);
+#pragma unroll
+        for (int i = 0; i < TN; i++) b[i] = *(const uint4 *)(bp + i * 32 * 128 + slot);
+    }
+};
+template <int TM, int TN> struct F8Step {
+    f8_v8bf a[TM], b[TN];
+    // operand i of step z of a chunk: A's tiles, then B's
+    template <int FA, int FB> __device__ __forceinline__ void convert(const F8Raw<TM, TN> &r, int z, int i) {
+        if (i < TM) a[i] = z ? f8_bf16x8<FA>(r.a[i].z, r.a[i].w) : f8_bf16x8<FA>(r.a[i].x, r.a[i].y);
+        else b[i - TM] = z ? f8_bf16x8<FB>(r.b[i - TM].z, r.b[i - TM].w) : f8_bf16x8<FB>(r.b[i - TM].x, r.b[i - TM].y);
+    }
+};
+// no instruction is scheduled across
+__device__ __forceinline__ void f8_pin() {
+#if defined(__HIP_DEVICE_COMPILE__)
+    __builtin_amdgcn_sched_barrier(0);
+#endif
+}
+
+// The scales of a block for a wave's tiles: sa_ at the lane's row of A, sb_ at the wave's first row of B.
+template <bool BROWS, int TM, int TN> struct F8Scales {
+    float a[TM], b;
+    f8_v4f rows[BROWS ? 4 * TN : 1];
+    __device__ __forceinline__ void read(const float *sa_, const float *sb_, int h) {
+#pragma unroll
+        for (int i = 0; i < TM; i++) a[i] = sa_[i * 32];
+        if constexpr (BROWS) {
+#pragma unroll
+            for (int q = 0; q < 4 * TN; q++) rows[q] = *(const f8_v4f *)(sb_ + 4 * h + 8 * q);
+        } else {
+            b = sb_[0];
+        }
+    }
+    // acc += part times the scales, for tile (im, in)
+    __device__ __forceinline__ void add(const f8_v16f &part, f8_v16f &acc, int im, int in) const {
+        const float one = a[im] * b;
+#pragma unroll
+        for (int i = 0; i < 16; i++)
+            acc[i] = __builtin_fmaf(part[i], BROWS ? a[im] * rows[BROWS ? 4 * in + i / 4 : 0][i % 4] : one, acc[i]);
+    }
+};
+
+// One block: the block before's products (part) are scaled into acc with the scales at sa, sb, then this block's are
+// computed.  The order keeps the matrix unit fed and is pinned, since the compiler's own puts the LDS reads next to
+// their use: a chunk is read a chunk ahead, and between one matrix instruction and the next stand the conversions of
+// an operand of the next step and, in the first step, the scaling of the tile that is overwritten next.
+template <int FA, int FB, bool BROWS, int TM, int TN, bool LATE>
+__device__ __forceinline__ void f8_block(const char *ap, const char *bp, const float *sa, const float *sb, int h, int swz,
+                                         f8_v16f (&part)[TN][TM], f8_v16f (&acc)[TN][TM]) {
+    constexpr int T = TM * TN, P = TM + TN;
+    F8Raw<TM, TN> r[2];
+    F8Step<TM, TN> s[2];
+    F8Scales<BROWS, TM, TN> sc;
+    r[0].read(ap, bp, 0, h, swz);
+    sc.read(sa, sb, h);
+    r[1].read(ap, bp, 1, h, swz);
+    f8_pin();
+#pragma unroll
+    for (int i = 0; i < P; i++) s[0].template convert<FA, FB>(r[0], 0, i);
+    if constexpr (LATE) sc.add(part[0][0], acc[0][0], 0, 0);
+#pragma unroll
+    for (int t = 0; t < 8; t++) {
+#pragma unroll
+        for (int i = 0; i < T; i++) {
+            const int in = i / TM, im = i % TM;
+            f8_pin();
+            part[in][im] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(s[t & 1].b[in], s[t & 1].a[im], t ? part[in][im] : f8_v16f{}, 0, 0, 0);
+            f8_pin();
+            if (i == 0 && (t == 1 || t == 3)) {
+                r[t == 3].read(ap, bp, t == 1 ? 2 : 3, h, swz);
+                f8_pin();
+            }
+            if (t < 7) {
+#pragma unroll
+                for (int o = i * P / T; o < (i + 1) * P / T; o++)
+                    s[(t + 1) & 1].template convert<FA, FB>(r[((t + 1) / 2) & 1], (t + 1) & 1, o);
+            }
+            if (LATE && t == 0 && i + 1 < T) sc.add(part[(i + 1) / TM][(i + 1) % TM], acc[(i + 1) / TM][(i + 1) % TM], (i + 1) % TM, (i + 1) / TM);
+        }
+    }
+    f8_pin();
+    if constexpr (!LATE) {
+#pragma unroll
+        for (int i = 0; i < T; i++) sc.add(part[i / TM][i % TM], acc[i / TM][i % TM], i % TM, i / TM);
+    }
+}
+// the last block's products into acc
+template <bool BROWS, int TM, int TN>
+__device__ __forceinline__ void f8_scale_add(const f8_v16f (&part)[TN][TM], const float *sa, const float *sb, int h,
+                                             f8_v16f (&acc)[TN][TM]) {
+    F8Scales<BROWS, TM, TN> sc;
+    sc.read(sa, sb, h);
+#pragma unroll
+    for (int in = 0; in < TN; in++)
+#pragma unroll
+        for (int im = 0; im < TM; im++) sc.add(part[in][im], acc[in][im], im, in);
+}
+
+// A wave's tiles as rows of 32 TN floats in LDS, in slots of four floats, slot s of row m at s ^ f8_turn(m): a column
+// of the accumulators' four-float pieces and a row both spread over the banks.
+template <int TN> __device__ __forceinline__ int f8_turn(int m) { return TN == 1 ? (m >> 1) & 7 : m & 15; }
+
+template <int TM, int TN>
+__device__ __forceinline__ void f8_put(float *t, const f8_v16f (&acc)[TN][TM], int l) {
+    static_assert(TN == 1 || TN == 2, "8 or 16 slots a row");
+    const int h = l >> 5;
+#pragma unroll
+    for (int im = 0; im < TM; im++) {
+        const int m = im * 32 + (l & 31);
+#pragma unroll
+        for (int in = 0; in < TN; in++)
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                f8_v4f v;
+                for (int e = 0; e < 4; e++) v[e] = acc[in][im][4 * q + e];
+                *(f8_v4f *)(t + m * 32 * TN + 4 * ((8 * in + 2 * q + h) ^ f8_turn<TN>(m))) = v;
+            }
+    }
+}
+
+// Writes rows [0, rows) of such a tile, summed over `parts` of them `stride` floats apart in order, to y's rows from
+// (m0, n0) on, plus the bias: whole rows of neighbouring floats by neighbouring threads.
+template <int TM, int TN>
+__device__ __forceinline__ void f8_store(const MatMulBlocksArgs &p, const float *t, int parts, int stride, int64_t m0, int64_t n0,
+                                         int thread, int threads) {
+    constexpr int W = 32 * TN;
+    const int rows = (int)std::min<int64_t>(32 * TM, p.m - m0), cols = (int)std::min<int64_t>(W, p.n - n0);
+    float *y = p.y + m0 * p.n + n0;
+    const float *bias = p.bias ? p.bias + n0 : nullptr;
+    if (p.n % 4 == 0 && ((uintptr_t)p.y & 15) == 0) {
+        for (int i = thread; i < rows * (W / 4); i += threads) {
+            const int m = i / (W / 4), s = i % (W / 4);
+            if (4 * s >= cols) continue;
+            const float *f = t + m * W + 4 * (s ^ f8_turn<TN>(m));
+            f8_v4f v = *(const f8_v4f *)f;
+            for (int k = 1; k < parts; k++) v += *(const f8_v4f *)(f + k * stride);
+            if (bias)
+                for (int e = 0; e < 4; e++) v[e] += bias[4 * s + e];
+            *(f8_v4f *)(y + m * p.n + 4 * s) = v;
+        }
+    } else {
+        for (int i = thread; i < rows * W; i += threads) {
+            const int m = i / W, n = i % W;
+            if (n >= cols) continue;
+            const float *f = t + m * W + 4 * ((n / 4) ^ f8_turn<TN>(m)) + n % 4;
+            float v = *f;
+            for (int k = 1; k < parts; k++) v += f[k * stride];
+            y[m * p.n + n] = bias ? v + bias[n] : v;
+        }
+    }
+}
+
+// A wave's own waits: all but its last N direct loads, and its LDS operations, are done; nothing that touches memory
+// moves across.
+template <int N> __device__ __forceinline__ void f8_wait() {
+    static_assert(N >= 0 && N < 64, "vmcnt range");
+#if defined(__HIP_DEVICE_COMPILE__)
+    __asm__ volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+#endif
+}
+__device__ __forceinline__ void f8_wait_lds() {
+#if defined(__HIP_DEVICE_COMPILE__)
+    __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#endif
+}
+__device__ __forceinline__ void f8_wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 template <int FA, int FB, bool BROWS, int TM, int TN, int WM, int WN, int S, int OCC>
 __global__ __launch_bounds__(64 * WM * WN, OCC) void k_matmul_blocks(MatMulBlocksArgs p, int tm, int tn) {
     constexpr int NW = WM * WN, BM = 32 * TM * WM, BN = 32 * TN * WN, R = BM + BN;
     constexpr int L = R / 8 / NW;               // 16-byte loads a wave and stage, of eight rows each
     constexpr int LS = (R / 64 + NW - 1) / NW;  // 4-byte loads of the rows' scales
-    static_assert(R % (8 * NW) == 0 && R % 64 == 0 && BM % 8 == 0 && BN <= 128, "whole wave loads");
-    constexpr int STAGE = R * 128 + LS * NW * 256;
+    static_assert(BM % (8 * NW) == 0 && BN % (8 * NW) == 0 && BM % 64 == 0 && BN % 64 == 0 && BN <= 128, "whole wave loads");
+    constexpr int STAGE = R * 128, SCALES = LS * NW * 64;
     __shared__ __attribute__((aligned(1024))) char sm[S][STAGE];
+    __shared__ __attribute__((aligned(256))) float sc[S + 1][SCALES];  // a block's scales are read one block later
     const int l = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = l >> 5;
 
     // tiles in groups of eight rows of tiles, contiguous ranges of them to each XCD (workgroups go round the 8 XCDs)
@@ -332,126 +488,206 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void k_matmul_blocks(MatMulBlock
         soff[i] = (uint32_t)(row * (int)kb * 4);
     }
     const int tail = (int)(p.k & 127);  // codes of a last block that is not whole
-    auto load = [&](int64_t j, char *st) {
-        const bool cut = tail && j == kb - 1;
+    auto load = [&](int64_t j, char *st, float *scl) {
+        if (tail && j == kb - 1) {
 #pragma unroll
-        for (int i = 0; i < L; i++) {
-            const bool is_a = 8 * (w + NW * i) < BM;  // uniform: eight rows are all A's or all B's
-            const uint8_t *base = (is_a ? abase : bbase) + 128 * j;
-            char *lds = st + 1024 * (w + NW * i);
-            if (!cut) {
-                f8_load_lds16(base, off[i], lds);
-            } else {
+            for (int i = 0; i < L; i++) {
                 const int r = 8 * (w + NW * i) + (l >> 3), c = (l & 7) ^ ((r >> 1) & 7);
-                if (16 * c < tail) f8_load_lds16(base, off[i], lds);
+                char *lds = st + 1024 * (w + NW * i);
+                if (16 * c < tail) f8_load_lds16((NW * i < BM / 8 ? abase : bbase) + 128 * j, off[i], lds);
                 else *(uint4 *)(lds + 16 * l) = uint4{0, 0, 0, 0};
             }
+        } else {
+#pragma unroll
+            for (int i = 0; i < L; i++)
+                f8_load_lds16((NW * i < BM / 8 ? abase : bbase) + 128 * j, off[i], st + 1024 * (w + NW * i));
         }
 #pragma unroll
-        for (int i = 0; i < LS; i++) {
-            const bool is_a = 64 * (w + NW * i) < BM;
-            f8_load_lds4((is_a ? sabase : sbbase) + j, soff[i], st + R * 128 + 256 * (w + NW * i));
-        }
+        for (int i = 0; i < LS; i++)
+            f8_load_lds4((64 * (w + NW * i) < BM ? sabase : sbbase) + j, soff[i], scl + 64 * (w + NW * i));
     };
 
-    f8_v16f acc[TN][TM] = {};
+    f8_v16f acc[TN][TM] = {}, part[TN][TM] = {};
     const int wm = w % WM, wn = w / WM;
     const int swz = ((l & 31) >> 1) & 7;
+    for (int i = threadIdx.x; i < SCALES; i += 64 * NW) sc[S][i] = 0.0f;  // before the first block: nothing times zero
     for (int s = 0; s < S - 1; s++)
-        if (s < kb) load(s, sm[s]);
-    int cur = 0;
+        if (s < kb) load(s, sm[s], sc[s]);
+    int cur = 0, scur = 0;
     for (int64_t j = 0; j < kb; j++) {
         // the last S - 2 stages ahead may still be landing; near the end there are fewer
         if (S > 2 && j + S - 2 < kb) f8_wait_barrier<(S - 2) * (L + LS)>();
         else f8_wait_barrier<0>();
-        const char *st = sm[cur];
-        if (j + S - 1 < kb) load(j + S - 1, sm[cur == 0 ? S - 1 : cur - 1]);
+        const char *st = sm[cur], *ap = st + (wm * TM * 32 + (l & 31)) * 128, *bp = st + (BM + wn * TN * 32 + (l & 31)) * 128;
+        const int before = scur == 0 ? S : scur - 1;  // the block before's scales
+        int ahead = scur + S - 1;
+        if (j + S - 1 < kb) load(j + S - 1, sm[cur == 0 ? S - 1 : cur - 1], sc[ahead > S ? ahead - S - 1 : ahead]);
         cur = cur + 1 == S ? 0 : cur + 1;
-        const char *ap = st + (wm * TM * 32 + (l & 31)) * 128, *bp = st + (BM + wn * TN * 32 + (l & 31)) * 128;
-        f8_v16f part[TN][TM] = {};
-#pragma unroll
-        for (int c = 0; c < 4; c++) {
-            uint4 va[TM], vb[TN];
-            const int slot = 16 * ((2 * c + h) ^ swz);
-#pragma unroll
-            for (int i = 0; i < TM; i++) va[i] = *(const uint4 *)(ap + i * 32 * 128 + slot);
-#pragma unroll
-            for (int i = 0; i < TN; i++) vb[i] = *(const uint4 *)(bp + i * 32 * 128 + slot);
-#pragma unroll
-            for (int z = 0; z < 2; z++) {
-                f8_v8bf a[TM], b[TN];
-#pragma unroll
-                for (int i = 0; i < TM; i++) a[i] = z ? f8_bf16x8<FA>(va[i].z, va[i].w) : f8_bf16x8<FA>(va[i].x, va[i].y);
-#pragma unroll
-                for (int i = 0; i < TN; i++) b[i] = z ? f8_bf16x8<FB>(vb[i].z, vb[i].w) : f8_bf16x8<FB>(vb[i].x, vb[i].y);
-#pragma unroll
-                for (int in_ = 0; in_ < TN; in_++)
-#pragma unroll
-                    for (int im = 0; im < TM; im++)
-                        part[in_][im] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(b[in_], a[im], part[in_][im], 0, 0, 0);
-            }
-        }
-        const float *sc = (const float *)(st + R * 128);
-        float sa[TM];
-#pragma unroll
-        for (int i = 0; i < TM; i++) sa[i] = sc[(wm * TM + i) * 32 + (l & 31)];
-#pragma unroll
-        for (int in_ = 0; in_ < TN; in_++) {
-            const float *sb = sc + BM + (wn * TN + in_) * 32 + 4 * h;
-#pragma unroll
-            for (int q = 0; q < 4; q++) {
-                f8_v4f b4;
-                if constexpr (BROWS) b4 = *(const f8_v4f *)(sb + 8 * q);
-#pragma unroll
-                for (int im = 0; im < TM; im++) {
-                    const float one = sa[im] * sc[BM + wn * TN * 32];
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const float f = BROWS ? sa[im] * b4[e] : one;
-                        acc[in_][im][4 * q + e] = __builtin_fmaf(part[in_][im][4 * q + e], f, acc[in_][im][4 * q + e]);
-                    }
-                }
-            }
-        }
+        scur = scur == S ? 0 : scur + 1;
+        const float *c = sc[before];
+        f8_block<FA, FB, BROWS, TM, TN, true>(ap, bp, c + wm * TM * 32 + (l & 31), c + BM + wn * TN * 32, h, swz, part, acc);
     }
-    const bool vec = p.n % 4 == 0 && ((uintptr_t)p.y & 15) == 0;
-#pragma unroll
-    for (int im = 0; im < TM; im++) {
-        const int64_t m = m0 + (wm * TM + im) * 32 + (l & 31);
-        if (m >= p.m) continue;
-#pragma unroll
-        for (int in_ = 0; in_ < TN; in_++)
-#pragma unroll
-            for (int q = 0; q < 4; q++) {
-                const int64_t n = n0 + (wn * TN + in_) * 32 + 8 * q + 4 * h;
-                f8_v4f v;
-                for (int e = 0; e < 4; e++) v[e] = acc[in_][im][4 * q + e];
-                if (vec) {
-                    if (n < p.n) {
-                        if (p.bias)
-                            for (int e = 0; e < 4; e++) v[e] += p.bias[n + e];
-                        *(f8_v4f *)(p.y + m * p.n + n) = v;
-                    }
-                } else {
-                    for (int e = 0; e < 4; e++)
-                        if (n + e < p.n) p.y[m * p.n + n + e] = p.bias ? v[e] + p.bias[n + e] : v[e];
-                }
-            }
+    if (kb) {
+        const float *c = sc[scur == 0 ? S : scur - 1];
+        f8_scale_add<BROWS>(part, c + wm * TM * 32 + (l & 31), c + BM + wn * TN * 32, h, acc);
     }
+    // the stages are done with: each wave's tiles go out through its part of them
+    f8_wait_barrier<0>();
+    float *t_ = (float *)&sm[0][0] + w * TM * TN * 1024;
+    static_assert(NW * TM * TN * 4096 <= S * STAGE, "room for the waves' tiles");
+    f8_put<TM, TN>(t_, acc, l);
+    f8_wave_sync();
+    f8_store<TM, TN>(p, t_, 1, 0, m0 + wm * TM * 32, n0 + wn * TN * 32, l, 64);
 }
 
-template <int FA, int FB, bool BROWS> static hipError_t matmul_blocks(const MatMulBlocksArgs &p, hipStream_t s) {
-    const bool chunks = p.k % 16 == 0 && p.k > 0 && (((uintptr_t)p.a | (uintptr_t)p.b) & 15) == 0 && p.k < (1 << 23);
-    const int64_t t128 = (p.m + 127) / 128 * ((p.n + 127) / 128), t64 = (p.m + 63) / 64 * ((p.n + 63) / 64);
-    if (chunks && t128 >= 256 && t128 < (1 << 26)) {
-        k_matmul_blocks<FA, FB, BROWS, 2, 2, 2, 2, 2, 2>
-            <<<(unsigned)((t128 + 7) / 8 * 8), 256, 0, s>>>(p, (int)((p.m + 127) / 128), (int)((p.n + 127) / 128));
-    } else if (chunks && p.m > 32 && t64 >= 256 && t64 < (1 << 26)) {
-        k_matmul_blocks<FA, FB, BROWS, 1, 1, 2, 2, 3, 3>
-            <<<(unsigned)((t64 + 7) / 8 * 8), 256, 0, s>>>(p, (int)((p.m + 63) / 64), (int)((p.n + 63) / 64));
+// ---- few tiles: waves over K ------------------------------------------------------------------------------------
+// Where a launch has too few tiles for the chip's workgroups, a workgroup takes one wave's tiles (TM x TN of 32x32) and
+// its W waves share the blocks of K (block j to wave j mod W), each with two stages of its own in LDS, so that no wave
+// waits for another until their sums are joined in order at the end.  LA: eight-row groups of A that are loaded (rows
+// from p.m on only reach results that are not stored).  CHUNKS: rows of whole aligned 16-byte chunks, loaded straight to
+// LDS; other rows go through registers, a block ahead too.
+template <int FA, int FB, bool BROWS, int TM, int TN, int LA, int MAXW, bool CHUNKS>
+__global__ __launch_bounds__(64 * MAXW) void k_matmul_blocks_thin(MatMulBlocksArgs p, int tm) {
+    constexpr int BM = 32 * TM, BN = 32 * TN, LB = BN / 8, L = LA + LB, LS = (BM + BN) / 64;
+    constexpr int STAGE = (BM + BN) * 128 + LS * 256;
+    __shared__ __attribute__((aligned(1024))) char sm[MAXW * 2 * STAGE];
+    const int l = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), W = blockDim.x >> 6, h = l >> 5;
+    char *mine = sm + w * 2 * STAGE;
+    // neighbouring workgroups take the row tiles of one range of B's rows
+    const int64_t m0 = (int64_t)(blockIdx.x % tm) * BM, n0 = (int64_t)(blockIdx.x / tm) * BN;
+    const int64_t kb = (p.k + 127) / 128;
+    const int row_n = BROWS ? 1 : 128;
+    const uint8_t *abase = p.a + m0 * p.k, *bbase = p.b + n0 * p.k;
+    const float *sabase = p.sa + m0 * kb, *sbbase = p.sb + n0 / row_n * kb;
+    const int rows_a = (int)std::min<int64_t>(p.m - m0, BM) - 1, rows_b = (int)std::min<int64_t>(p.n - n0, BN) - 1;
+    const int tail = (int)(p.k & 127);
+
+    uint32_t off[L], soff[LS];
+#pragma unroll
+    for (int i = 0; i < L; i++) {
+        const int r = 8 * (i < LA ? i : i - LA + BM / 8) + (l >> 3), c = (l & 7) ^ ((r >> 1) & 7);
+        off[i] = (uint32_t)((i < LA ? min(r, rows_a) : min(r - BM, rows_b)) * (int)p.k + 16 * c);
+    }
+#pragma unroll
+    for (int i = 0; i < LS; i++) {
+        const int r = 64 * i + l;
+        soff[i] = (uint32_t)((r < BM ? min(r, rows_a) : min(r - BM, rows_b) / row_n) * (int)kb * 4);
+    }
+    auto scales = [&](int64_t j, char *st) {
+#pragma unroll
+        for (int i = 0; i < LS; i++) {
+            if constexpr (BM % 64 == 0) {
+                f8_load_lds4((64 * i < BM ? sabase : sbbase) + j, soff[i], st + (BM + BN) * 128 + 256 * i);
+            } else {  // the first half of the lanes A's rows, the second B's
+                if (l < BM) f8_load_lds4(sabase + j, soff[i], st + (BM + BN) * 128);
+                else f8_load_lds4(sbbase + j, soff[i], st + (BM + BN) * 128);
+            }
+        }
+    };
+    constexpr int NL = L + (BM % 64 == 0 ? LS : 2);  // direct loads a stage
+    auto load = [&](int64_t j, char *st) {
+        const bool cut = tail && j == kb - 1;
+#pragma unroll
+        for (int i = 0; i < L; i++) {
+            const int g = i < LA ? i : i - LA + BM / 8;
+            const uint8_t *base = (i < LA ? abase : bbase) + 128 * j;
+            if (!cut) {
+                f8_load_lds16(base, off[i], st + 1024 * g);
+            } else {
+                const int r = 8 * g + (l >> 3), c = (l & 7) ^ ((r >> 1) & 7);
+                if (16 * c < tail) f8_load_lds16(base, off[i], st + 1024 * g);
+                else *(uint4 *)(st + 1024 * g + 16 * l) = uint4{0, 0, 0, 0};
+            }
+        }
+        scales(j, st);
+    };
+    uint4 reg[CHUNKS ? 1 : L];
+    auto fetch = [&](int64_t j) {
+#pragma unroll
+        for (int i = 0; i < (CHUNKS ? 0 : L); i++) {
+            const int g = i < LA ? i : i - LA + BM / 8, r = 8 * g + (l >> 3), c = (l & 7) ^ ((r >> 1) & 7);
+            const uint8_t *row = (i < LA ? abase : bbase) + (int64_t)off[i] - 16 * c;
+            reg[i] = f8_load16(row, 128 * (int)j + 16 * c, (int)p.k);
+        }
+    };
+    auto drop = [&](int64_t j, char *st) {
+#pragma unroll
+        for (int i = 0; i < (CHUNKS ? 0 : L); i++) {
+            const int g = i < LA ? i : i - LA + BM / 8, r = 8 * g + (l >> 3), c = (l & 7) ^ ((r >> 1) & 7);
+            *(uint4 *)(st + 1024 * g + 16 * l) = j == kb - 1 ? f8_tail16(reg[i], 128 * (int)j + 16 * c, (int)p.k) : reg[i];
+        }
+    };
+
+    f8_v16f acc[TN][TM] = {}, part[TN][TM];
+    const int swz = ((l & 31) >> 1) & 7;
+    auto block = [&](const char *st) {
+        const float *sc = (const float *)(st + (BM + BN) * 128);
+        f8_block<FA, FB, BROWS, TM, TN, false>(st + (l & 31) * 128, st + (BM + (l & 31)) * 128, sc + (l & 31), sc + BM, h, swz, part, acc);
+    };
+    if constexpr (CHUNKS) {
+        if (w < kb) load(w, mine);
+        if (w + W < kb) load(w + W, mine + STAGE);
+        int cur = 0;
+        for (int64_t j = w; j < kb; j += W) {
+            char *st = mine + cur * STAGE;
+            if (j + W < kb) f8_wait<NL>();
+            else f8_wait<0>();
+            block(st);
+            f8_wait_lds();  // this stage has been read
+            if (j + 2 * W < kb) load(j + 2 * W, st);
+            cur ^= 1;
+        }
     } else {
-        const int64_t tiles = (p.m + 31) / 32 * ((p.n + 31) / 32);
-        k_matmul_blocks_small<FA, FB, BROWS><<<(unsigned)tiles, 256, 0, s>>>(p);
+        if (w < kb) fetch(w);
+        for (int64_t j = w; j < kb; j += W) {
+            f8_wait_lds();
+            drop(j, mine);
+            scales(j, mine);
+            if (j + W < kb) fetch(j + W);
+            f8_wait<0>();
+            block(mine);
+        }
+    }
+    // every wave's sums in its own stage, joined in the waves' order
+    f8_wait_lds();
+    f8_put<TM, TN>((float *)mine, acc, l);
+    __syncthreads();
+    f8_store<TM, TN>(p, (const float *)sm, W, 2 * STAGE / 4, m0, n0, threadIdx.x, blockDim.x);
+}
+
+template <int FA, int FB, bool BROWS, int TM, int TN, int LA, int MAXW>
+static void thin(const MatMulBlocksArgs &p, bool chunks, hipStream_t s) {
+    const int64_t tm = (p.m + 32 * TM - 1) / (32 * TM), tn = (p.n + 32 * TN - 1) / (32 * TN);
+    const unsigned threads = 64 * (unsigned)std::max<int64_t>(1, std::min<int64_t>(MAXW, (p.k + 127) / 128));
+    if (chunks) k_matmul_blocks_thin<FA, FB, BROWS, TM, TN, LA, MAXW, true><<<(unsigned)(tm * tn), threads, 0, s>>>(p, (int)tm);
+    else k_matmul_blocks_thin<FA, FB, BROWS, TM, TN, LA, MAXW, false><<<(unsigned)(tm * tn), threads, 0, s>>>(p, (int)tm);
+}
+
+// The kernel of a product by its tiles of Y, one workgroup each, against the chip's 256 CUs (us on one device, e4m3):
+//   128x128 from 256 of them on: [512,768]x[30522,768] 39 against 48 in tiles of 64x64, 8192x4096x8192 492 against 640;
+//     4096x768x768, 192 of them, 13.0 against 12.5
+//   64x64 from 257 on: 2048x1024x1024 11.4 against 12.9 with waves over K; 1024x1024x1024, 256 of them, 8.6 against 7.5
+//   64x64 with waves over K from 128 on, and for rows that are not whole chunks: 788x768x768 6.9 against 7.4 in tiles
+//     of 32x32; 333x1232x1001, 96 of them, 12.1 against 7.8
+//   32x32 with waves over K: eight waves up to 256 of them (64x4096x4096 9.6 against 10.0), more with four, two
+//     workgroups a CU (788x768x768 7.4 against 8.9); of at most eight rows only those of A are read.
+template <int FA, int FB, bool BROWS> static hipError_t matmul_blocks(const MatMulBlocksArgs &p, hipStream_t s) {
+    const bool chunks = p.k % 16 == 0 && (((uintptr_t)p.a | (uintptr_t)p.b) & 15) == 0;
+    auto tiles = [&](int64_t b) { return (p.m + b - 1) / b * ((p.n + b - 1) / b); };
+    if (chunks && tiles(128) >= 256) {
+        k_matmul_blocks<FA, FB, BROWS, 2, 2, 2, 2, 2, 2>
+            <<<(unsigned)((tiles(128) + 7) / 8 * 8), 256, 0, s>>>(p, (int)((p.m + 127) / 128), (int)((p.n + 127) / 128));
+    } else if (chunks && p.m > 32 && tiles(64) > 256) {
+        k_matmul_blocks<FA, FB, BROWS, 1, 1, 2, 2, 3, 3>
+            <<<(unsigned)((tiles(64) + 7) / 8 * 8), 256, 0, s>>>(p, (int)((p.m + 63) / 64), (int)((p.n + 63) / 64));
+    } else if (p.m > 32 && tiles(64) >= 128) {
+        thin<FA, FB, BROWS, 2, 2, 8, 4>(p, chunks, s);
+    } else if (tiles(32) <= 256) {
+        if (p.m <= 8) thin<FA, FB, BROWS, 1, 1, 1, 8>(p, chunks, s);
+        else thin<FA, FB, BROWS, 1, 1, 4, 8>(p, chunks, s);
+    } else {
+        if (p.m <= 8) thin<FA, FB, BROWS, 1, 1, 1, 4>(p, chunks, s);
+        else thin<FA, FB, BROWS, 1, 1, 4, 4>(p, chunks, s);
     }
     return hipGetLastError();
 }

@@ -243,7 +243,9 @@ struct QuantizeArgs {
 hipError_t launch_quantize_blocks(const QuantizeArgs &a, hipStream_t s);
 
 // MatMulBlocks: y[m, n] = a[m, k] b[n, k]^T of 8-bit codes (fmt_a, fmt_b) with scales sa [m, ceil(k / 128)] and sb
-// [n or ceil(n / 128), ceil(k / 128)] (b_rows 1 or 128), plus bias[n] unless null.  m, n > 0 and below 2^31.
+// [n or ceil(n / 128), ceil(k / 128)] (b_rows 1 or 128), plus bias[n] unless null.  m, n > 0 and below 2^31, k below kMatMulBlocksK (row offsets within a
+// tile are 32 bits), at most 2^23 tiles of 32x32.
+constexpr int64_t kMatMulBlocksK = 1 << 23;
 struct MatMulBlocksArgs {
     const uint8_t *a, *b;
     const float *sa, *sb, *bias;

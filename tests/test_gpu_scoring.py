@@ -127,7 +127,9 @@ def product(hip, a, sa, fa, b, sb, fb, bias=None, offset=0):
 
 SHAPES = [(1, 1, 1), (1, 128, 128), (1, 384, 384), (2, 129, 33), (7, 127, 130), (31, 512, 96), (33, 640, 257), (64, 256, 64),
           (65, 2048, 100), (1, 4096, 515), (16, 16, 16), (100, 1111, 77), (129, 768, 384), (128, 144, 1000), (257, 400, 300),
-          (300, 384, 513), (1000, 272, 129), (512, 1536, 640), (1, 20000, 5)]
+          (300, 384, 513), (1000, 272, 129), (512, 1536, 640), (1, 20000, 5),
+          (3, 256, 8300), (3, 77, 8300), (200, 333, 1500), (500, 384, 1030), (500, 301, 1030), (1040, 400, 1030), (1088, 256, 1088),
+          (2000, 272, 2100), (2049, 128, 2051), (2000, 131, 2100), (2048, 640, 2048)]
 
 
 @pytest.mark.parametrize("m,k,n", SHAPES)
@@ -143,7 +145,8 @@ def test_matmul(hip, m, k, n, by_row):
 
 @pytest.mark.parametrize("fa", [E4M3, E5M2])
 @pytest.mark.parametrize("fb", [E4M3, E5M2])
-@pytest.mark.parametrize("m,k,n", [(1, 300, 70), (40, 256, 130), (260, 384, 200)])
+@pytest.mark.parametrize("m,k,n", [(1, 300, 70), (40, 256, 130), (260, 384, 200), (500, 144, 1030), (1040, 144, 1030),
+                                   (2000, 144, 2100)])
 def test_matmul_every_pair_of_types_and_alignment(hip, fa, fb, m, k, n):
     rng = np.random.default_rng([fa, fb, m])
     (a, sa), (b, sb) = operand(rng, m, k, fa, True), operand(rng, n, k, fb, False)
@@ -152,7 +155,8 @@ def test_matmul_every_pair_of_types_and_alignment(hip, fa, fb, m, k, n):
         near(product(hip, a, sa, fa, b, sb, fb, offset=offset), *want)
 
 
-@pytest.mark.parametrize("m,k,n", [(1, 1024, 128), (5, 130, 260), (70, 384, 33), (256, 640, 384), (513, 128, 1025)])
+@pytest.mark.parametrize("m,k,n", [(1, 1024, 128), (5, 130, 260), (70, 384, 33), (256, 640, 384), (513, 128, 1025),
+                                   (1040, 640, 1030), (2000, 400, 2100)])
 @pytest.mark.parametrize("by_row", [False, True])
 def test_matmul_is_exact_where_float_is(hip, m, k, n, by_row):
     """Small whole values with scales that are powers of two: every sum is a float, whatever its order."""
@@ -166,7 +170,7 @@ def test_matmul_is_exact_where_float_is(hip, m, k, n, by_row):
     assert np.array_equal(product(hip, a, sa, E4M3, b, sb, E4M3, bias), want)
 
 
-@pytest.mark.parametrize("m,n", [(3, 40), (200, 300)])
+@pytest.mark.parametrize("m,n", [(3, 40), (200, 300), (520, 1030), (1040, 1030), (2000, 2100)])
 def test_matmul_special_values(hip, m, n):
     """NaN and infinite codes reach the rows and columns that hold them and no others; scales of zero count."""
     k = 272
@@ -207,7 +211,7 @@ def test_matmul_leading_axes_and_empty(hip):
 def test_matmul_writes_its_own_rows_only(hip):
     """The storage behind the last row, and the rows of a larger buffer, stay as they were."""
     rng = np.random.default_rng(9)
-    for m, k, n in ((5, 384, 130), (130, 256, 260)):
+    for m, k, n in ((5, 384, 130), (130, 256, 260), (500, 384, 1031), (1033, 144, 1030), (2000, 272, 2102)):
         (a, sa), (b, sb) = operand(rng, m, k, E4M3, True), operand(rng, n, k, E4M3, False)
         big = dev(hip, np.full((m + 2, n), 7.0, np.float32))
         out = hip.DeviceTensor.wrap(big.h.data + 4 * n, (m, n), np.float32, 4 * m * n, keepalive=big)
