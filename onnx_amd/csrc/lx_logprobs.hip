@@ -11,7 +11,7 @@
 //
 // The most probable tokens come from the same pass: each thread keeps the largest of the four-logit units it reads,
 // and the k-th largest over 64 groups of threads bounds the k-th largest logit from below (k distinct units reach
-// it).  Only threads whose own largest reaches the bound read their logits again, and only logits that reach it
+// it).  Only the logits of threads whose own largest reaches the bound are read again, and only logits that reach it
 // are ranked, by counting; equal logits rank by index.
 #include <hip/hip_runtime.h>
 
@@ -22,7 +22,7 @@
 
 namespace lx {
 
-constexpr int kLpBlock = 256, kLpCap = 2048, kLpSplit = 64;
+constexpr int kLpBlock = 256, kLpSplit = 64;
 
 struct LpStat {
     float m, r, t, n;
@@ -113,132 +113,191 @@ __device__ __forceinline__ void stat_add(LpStat &s, const float4 *f, int units) 
     }
 }
 
-// The k largest of `count` distinct keys into out, largest first (all threads of the block; count <= what buf holds).
-__device__ __forceinline__ void rank_keys(const uint64_t *buf, int count, int k, uint64_t *out) {
-    for (int c = threadIdx.x; c < count; c += kLpBlock) {
+// A row is a team's work: one wave's (TEAM 64, four rows a workgroup) or the whole workgroup's (TEAM 256).
+template <int TEAM> __device__ __forceinline__ void team_sync() {
+    if constexpr (TEAM == 64) {
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    } else {
+        __syncthreads();
+    }
+}
+
+template <int TEAM> struct LpShared {
+    static constexpr int kCap = 4 * TEAM + 2 * TEAM + 512;  // a round's keys, and those kept or waiting
+    uint64_t buf[kCap + 8];
+    uint64_t group[TEAM];
+    uint64_t top[kLogProbsTop];
+    uint32_t winner[TEAM];
+    LpStat wave[TEAM / 64];
+    uint64_t bound;
+    int count, winners;
+};
+
+// The k largest of `count` distinct keys into out, largest first (buf has room for eight more; the team's writes to it
+// are done).
+template <int TEAM> __device__ __forceinline__ void rank_keys(uint64_t *buf, int count, int k, uint64_t *out, int lane) {
+    if (lane < 8) buf[count + lane] = 0;
+    team_sync<TEAM>();
+    for (int c = lane; c < count; c += TEAM) {
         const uint64_t mine = buf[c];
         int rank = 0;
-        for (int j = 0; j < count && rank < k; j++) rank += buf[j] > mine;
+        for (int j = 0; j < count; j += 8) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) rank += buf[j + i] > mine;
+        }
         if (rank < k) out[rank] = mine;
     }
 }
 
-struct LpShared {
-    uint64_t buf[kLpCap];
-    uint64_t group[kLpBlock];
-    uint64_t top[kLogProbsTop];
-    LpStat wave[4];
-    uint64_t bound;
-    int count;
-};
-
-// the k-th largest of the wave's 64 keys, distinct but for zeros (none): zero if fewer than k are there
-__device__ __forceinline__ uint64_t wave_kth(uint64_t g, int k) {
-    int rank = 0;
-    for (int j = 0; j < 64; j++) {
-        const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)g, j), hi = __builtin_amdgcn_readlane((int)(g >> 32), j);
-        rank += ((uint64_t)hi << 32 | lo) > g;
-    }
-    const uint64_t at = __ballot(g != 0 && rank == k - 1);
-    if (!at) return 0;
-    const int j = __builtin_ctzll(at);
+__device__ __forceinline__ uint64_t lane_key(uint64_t g, int j) {
     const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)g, j), hi = __builtin_amdgcn_readlane((int)(g >> 32), j);
     return (uint64_t)hi << 32 | lo;
 }
 
+// the k-th largest of the wave's keys, distinct but for zeros (none): zero if fewer than k are there
+__device__ __forceinline__ uint64_t wave_kth(uint64_t g, int k) {
+    int rank = 0;
+#pragma unroll
+    for (int j = 0; j < 64; j++) rank += lane_key(g, j) > g;
+    const uint64_t at = __ballot(g != 0 && rank == k - 1);
+    return at ? lane_key(g, __builtin_ctzll(at)) : 0;
+}
+// the same of two keys a lane
+__device__ __forceinline__ uint64_t wave_kth2(uint64_t g0, uint64_t g1, int k) {
+    int r0 = 0, r1 = 0;
+#pragma unroll 8
+    for (int j = 0; j < 64; j++) {
+        const uint64_t a = lane_key(g0, j), b = lane_key(g1, j);
+        r0 += (a > g0) + (b > g0);
+        r1 += (a > g1) + (b > g1);
+    }
+    const uint64_t at0 = __ballot(g0 != 0 && r0 == k - 1), at1 = __ballot(g1 != 0 && r1 == k - 1);
+    return at0 ? lane_key(g0, __builtin_ctzll(at0)) : at1 ? lane_key(g1, __builtin_ctzll(at1)) : 0;
+}
+
 // sh.top[0 .. k) = the k largest keys of units [u0, u1) of the row, zeros where there are fewer; `best` is this
-// thread's largest unit (value, unit), zero if none.
-__device__ void block_top(const LpRow &row, uint32_t u0, uint32_t u1, int k, uint64_t best, LpShared &sh) {
-    sh.group[threadIdx.x] = best;
-    if (threadIdx.x < kLogProbsTop) sh.top[threadIdx.x] = 0;
-    if (threadIdx.x == 0) sh.count = 0;
-    __syncthreads();
-    if (threadIdx.x < 64) {
-        uint64_t g = 0;
-        for (int w = 0; w < kLpBlock / 64; w++) g = std::max(g, sh.group[64 * w + threadIdx.x]);
-        g = wave_kth(g, k);
-        if (threadIdx.x == 0) sh.bound = g;
-    }
-    __syncthreads();
-    const uint64_t bound = sh.bound;
-    const bool search = best >= bound;
-    if (search) {
-        for (uint32_t u = u0 + threadIdx.x; u < u1; u += kLpBlock) {
-            const float4 f = row.load(u);
-            const float *p = &f.x;
-            for (int i = 0; i < 4; i++)
-                if (lp_key(p[i], u) >= bound && row.inside(u, i)) {
-                    const int at = atomicAdd(&sh.count, 1);
-                    if (at < kLpCap) sh.buf[at] = lp_key(p[i], 4 * u - row.off + i);
-                }
+// thread's largest unit (value, unit) of those u0 + lane + TEAM i, zero if none.
+template <int TEAM>
+__device__ void team_top(const LpRow &row, uint32_t u0, uint32_t u1, int k, uint64_t best, LpShared<TEAM> &sh, int lane) {
+    using Sh = LpShared<TEAM>;
+    sh.group[lane] = best;
+    if (lane < kLogProbsTop) sh.top[lane] = 0;
+    if (lane == 0) sh.count = sh.winners = 0;
+    team_sync<TEAM>();
+    if (lane < 64) {
+        uint64_t g;
+        if constexpr (TEAM == 64) {
+            g = wave_kth(best, k);
+        } else if (k > 32) {  // two keys a lane: 64 of 64 groups would let many logits past the bound
+            g = wave_kth2(std::max(sh.group[lane], sh.group[lane + 64]), std::max(sh.group[lane + 128], sh.group[lane + 192]), k);
+        } else {
+            g = wave_kth(std::max(std::max(sh.group[lane], sh.group[lane + 64]), std::max(sh.group[lane + 128], sh.group[lane + 192])), k);
         }
+        if (lane == 0) sh.bound = g;
     }
-    __syncthreads();
+    team_sync<TEAM>();
+    const uint64_t bound = sh.bound;
+    if (best >= bound) sh.winner[atomicAdd(&sh.winners, 1)] = lane;
+    team_sync<TEAM>();
+    // the winners' units, shared out over the team
+    const uint32_t winners = sh.winners, total = winners * ((u1 - u0 + TEAM - 1) / TEAM);
+    auto unit = [&](uint32_t i) { return u0 + sh.winner[i % winners] + TEAM * (i / winners); };
+    auto offer = [&](const float4 &f, uint32_t u, auto &&take) {
+        const float *p = &f.x;
+        for (int i = 0; i < 4; i++)
+            if (lp_key(p[i], u) >= bound && row.inside(u, i)) take(lp_key(p[i], 4 * u - row.off + i));
+    };
+    for (uint32_t i = lane; i < total; i += 4 * TEAM) {
+        float4 f[4];
+        uint32_t u[4];
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            u[c] = i + c * TEAM < total ? unit(i + c * TEAM) : u1;
+            if (u[c] < u1) f[c] = row.load(u[c]);
+        }
+#pragma unroll
+        for (int c = 0; c < 4; c++)
+            if (u[c] < u1)
+                offer(f[c], u[c], [&](uint64_t key) {
+                    const int at = atomicAdd(&sh.count, 1);
+                    if (at < Sh::kCap) sh.buf[at] = key;
+                });
+    }
+    team_sync<TEAM>();
     int count = sh.count;
-    if (count <= kLpCap) {
-        rank_keys(sh.buf, count, k, sh.top);
-        __syncthreads();
+    if (count <= Sh::kCap) {
+        rank_keys<TEAM>(sh.buf, count, k, sh.top, lane);
+        team_sync<TEAM>();
         return;
     }
     // more than the buffer holds (few distinct logits, or sorted ones): by rounds, the k largest so far kept
-    __syncthreads();
-    if (threadIdx.x == 0) sh.count = 0;
-    __syncthreads();
-    for (uint32_t u = u0; u < u1; u += kLpBlock) {
-        if (search && u + threadIdx.x < u1) {
-            const float4 f = row.load(u + threadIdx.x);
-            const float *p = &f.x;
+    team_sync<TEAM>();
+    if (lane == 0) sh.count = 0;
+    team_sync<TEAM>();
+    for (uint32_t i = 0; i < total; i += TEAM) {
+        const uint32_t u = i + lane < total ? unit(i + lane) : u1;
+        if (u < u1) {
             const uint64_t least = sh.top[k - 1];
-            for (int i = 0; i < 4; i++) {
-                const uint64_t key = lp_key(p[i], 4 * (u + threadIdx.x) - row.off + i);
-                if (lp_key(p[i], u + threadIdx.x) >= bound && row.inside(u + threadIdx.x, i) && key > least)
-                    sh.buf[atomicAdd(&sh.count, 1)] = key;
-            }
+            offer(row.load(u), u, [&](uint64_t key) {
+                if (key > least) sh.buf[atomicAdd(&sh.count, 1)] = key;
+            });
         }
-        __syncthreads();
+        team_sync<TEAM>();
         count = sh.count;
-        // room for the next round's 4 * kLpBlock keys, or the last round
-        if (count > kLpCap - 4 * kLpBlock - kLogProbsTop || u + kLpBlock >= u1) {
-            if (threadIdx.x < k && sh.top[threadIdx.x]) sh.buf[count + threadIdx.x] = sh.top[threadIdx.x];
-            __syncthreads();
+        // room for the next round's 4 TEAM keys, or the last round
+        if (count > Sh::kCap - 4 * TEAM - kLogProbsTop || i + TEAM >= total) {
             int kept = 0;
             while (kept < k && sh.top[kept]) kept++;
-            __syncthreads();
-            rank_keys(sh.buf, count + kept, k, sh.top);
-            if (threadIdx.x == 0) sh.count = 0;
+            if (lane < kept) sh.buf[count + lane] = sh.top[lane];
+            team_sync<TEAM>();
+            rank_keys<TEAM>(sh.buf, count + kept, k, sh.top, lane);
+            if (lane == 0) sh.count = 0;
         }
-        __syncthreads();
+        team_sync<TEAM>();
     }
 }
+
+// The given token's logit, read by the team's first lane before the row's pass, behind which its latency hides.
+struct LpAsked {
+    int64_t id;
+    float x;
+    __device__ __forceinline__ LpAsked(const LogProbsArgs &a, int64_t row, bool mine) : id(-1), x(0.0f) {
+        if (!a.ids || !mine) return;
+        id = a.ids_dtype == kInt64 ? ((const int64_t *)a.ids)[row] : (int64_t)((const int32_t *)a.ids)[row];
+        if (id >= 0 && id < a.v) x = a.x[row * a.v + id];
+    }
+};
 
 // a row's outputs from its sums and sorted keys
-__device__ __forceinline__ void lp_finish(const LogProbsArgs &a, int64_t row, const LpStat &s, const uint64_t *top) {
+template <int TEAM>
+__device__ __forceinline__ void lp_finish(const LogProbsArgs &a, int64_t row, const LpStat &s, const LpAsked &q,
+                                          const uint64_t *top, int lane) {
     const float ls = s.n > 0.0f ? log1pf((s.n - 1.0f) + s.r) : __builtin_nanf("");
-    if (threadIdx.x == 0) {
-        if (a.ids) {
-            const int64_t id = a.ids_dtype == kInt64 ? ((const int64_t *)a.ids)[row] : (int64_t)((const int32_t *)a.ids)[row];
-            float lp = 0.0f;
-            if (id >= a.v) lp = __builtin_nanf("");
-            else if (id >= 0) lp = (a.x[row * a.v + id] - s.m) - ls;
-            a.lp[row] = lp;
-        }
+    if (lane == 0) {
+        if (a.ids) a.lp[row] = q.id < 0 ? 0.0f : q.id >= a.v ? __builtin_nanf("") : (q.x - s.m) - ls;
         if (a.h) a.h[row] = ls + s.t / (s.n + s.r);
     }
-    if (threadIdx.x < a.top) {
-        const uint64_t key = top[threadIdx.x];
-        a.top_ids[row * a.top + threadIdx.x] = (int64_t)(uint32_t)~(uint32_t)key;
-        a.top_lp[row * a.top + threadIdx.x] = (lp_value((uint32_t)(key >> 32)) - s.m) - ls;
+    if (lane < a.top) {
+        const uint64_t key = top[lane];
+        a.top_ids[row * a.top + lane] = (int64_t)(uint32_t)~(uint32_t)key;
+        a.top_lp[row * a.top + lane] = (lp_value((uint32_t)(key >> 32)) - s.m) - ls;
     }
 }
 
-// One workgroup a part of a row (SPLIT: kLpSplit parts at most, their sums and keys to a.part) or a whole row.
-template <bool TOP, bool SPLIT>
+// A part of a row (SPLIT: kLpSplit parts at most, their sums and keys to a.part) or a whole row for each team.
+template <int TEAM, bool TOP, bool SPLIT>
 __global__ __launch_bounds__(kLpBlock) void k_logprobs(LogProbsArgs a, int split) {
-    __shared__ LpShared sh;
+    constexpr int TEAMS = kLpBlock / TEAM;
+    __shared__ LpShared<TEAM> shared[TEAMS];
+    const int lane = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
+    LpShared<TEAM> &sh = shared[team];
     const int64_t total = a.t * split;
-    for (int64_t b = blockIdx.x; b < total; b += gridDim.x) {
+    for (int64_t b = (int64_t)blockIdx.x * TEAMS + team; b < total; b += (int64_t)gridDim.x * TEAMS) {
         const int64_t r = SPLIT ? b / split : b;
         const int part = SPLIT ? (int)(b - r * split) : 0;
+        const LpAsked asked(a, r, !SPLIT && lane == 0);
         const LpRow row(a.x + r * a.v, a.v);
         const uint32_t per = SPLIT ? (uint32_t)(((a.v + 6) / 4 + split - 1) / split) : row.units;
         const uint32_t u0 = std::min(row.units, part * per), u1 = std::min(row.units, u0 + per);
@@ -246,76 +305,89 @@ __global__ __launch_bounds__(kLpBlock) void k_logprobs(LogProbsArgs a, int split
         LpStat s = {-__builtin_inff(), 0.0f, 0.0f, 0.0f};
         float best = -__builtin_inff();
         uint32_t best_u = 0;
-        for (uint32_t u = u0 + threadIdx.x; u < u1; u += 4 * kLpBlock) {
+        for (uint32_t u = u0 + lane; u < u1; u += 4 * TEAM) {
             float4 f[4];
 #pragma unroll
-            for (int c = 0; c < 4; c++) f[c] = u + c * kLpBlock < u1 ? row.load(u + c * kLpBlock) : none;
+            for (int c = 0; c < 4; c++) f[c] = u + c * TEAM < u1 ? row.load(u + c * TEAM) : none;
             if constexpr (TOP) {
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
                     const float m = max4(f[c]);
-                    best_u = m > best ? u + c * kLpBlock : best_u;
+                    best_u = m > best ? u + c * TEAM : best_u;
                     best = fmaxf(best, m);
                 }
             }
             stat_add(s, f, 4);
         }
         s = stat_wave(s);
-        __syncthreads();  // the previous row's use of sh
-        if ((threadIdx.x & 63) == 0) sh.wave[threadIdx.x >> 6] = s;
-        __syncthreads();
-        s = stat_merge(stat_merge(sh.wave[0], sh.wave[1]), stat_merge(sh.wave[2], sh.wave[3]));
-        if constexpr (TOP)
-            block_top(row, u0, u1, a.top, best > -__builtin_inff() ? lp_key(best, best_u) : 0, sh);
-        if constexpr (SPLIT) {
-            if (threadIdx.x == 0) ((LpStat *)a.part)[b] = s;
-            if (TOP && threadIdx.x < a.top) ((uint64_t *)((LpStat *)a.part + total))[b * a.top + threadIdx.x] = sh.top[threadIdx.x];
-        } else {
-            lp_finish(a, r, s, sh.top);
+        if constexpr (TEAM > 64) {
+            __syncthreads();  // the previous row's use of sh
+            if ((threadIdx.x & 63) == 0) sh.wave[threadIdx.x >> 6] = s;
+            __syncthreads();
+            s = stat_merge(stat_merge(sh.wave[0], sh.wave[1]), stat_merge(sh.wave[2], sh.wave[3]));
         }
+        if constexpr (TOP)
+            team_top<TEAM>(row, u0, u1, a.top, best > -__builtin_inff() ? lp_key(best, best_u) : 0, sh, lane);
+        if constexpr (SPLIT) {
+            if (lane == 0) ((LpStat *)a.part)[b] = s;
+            if (TOP && lane < a.top) ((uint64_t *)((LpStat *)a.part + total))[b * a.top + lane] = sh.top[lane];
+        } else {
+            lp_finish<TEAM>(a, r, s, asked, sh.top, lane);
+        }
+        if constexpr (TOP) team_sync<TEAM>();  // the next row's use of sh.top
     }
 }
 
 // Joins a row's parts.
 template <bool TOP>
 __global__ __launch_bounds__(kLpBlock) void k_logprobs_join(LogProbsArgs a, int split) {
-    __shared__ uint64_t buf[TOP ? kLpSplit * kLogProbsTop : 1];
+    __shared__ uint64_t buf[TOP ? kLpSplit * kLogProbsTop + 8 : 1];
     __shared__ uint64_t top[kLogProbsTop];
     __shared__ uint64_t bound;
     __shared__ int count;
     for (int64_t r = blockIdx.x; r < a.t; r += gridDim.x) {
         const int lane = threadIdx.x & 63;
+        const LpAsked asked(a, r, threadIdx.x == 0);
         LpStat s = {-__builtin_inff(), 0.0f, 0.0f, 0.0f};
         if (lane < split) s = ((const LpStat *)a.part)[r * split + lane];
+        constexpr int kKeys = 4;  // read before the bound is known; there are seldom more than 4 a thread
+        uint64_t key[kKeys], first = 0;
+        const int j = TOP ? (a.top + split - 1) / split : 1;
+        const uint64_t *keys = (const uint64_t *)((const LpStat *)a.part + a.t * split) + r * split * a.top;
+        if constexpr (TOP) {
+            first = lane < split ? keys[lane * a.top + j - 1] : j == 1 ? 0 : ~0ull;
+#pragma unroll
+            for (int i = 0; i < kKeys; i++)
+                key[i] = threadIdx.x + i * kLpBlock < split * a.top ? keys[threadIdx.x + i * kLpBlock] : 0;
+        }
         s = stat_wave(s);
         if constexpr (TOP) {
-            const uint64_t *keys = (const uint64_t *)((const LpStat *)a.part + a.t * split) + r * split * a.top;
             __syncthreads();  // the previous row's use of the shared arrays
             if (threadIdx.x == 0) count = 0;
             if (threadIdx.x < 64) {
                 // k keys of the parts' sorted lists reach the bound: the k-th of the first ones, or every list's j-th
-                const int j = (a.top + split - 1) / split;
-                uint64_t g = lane < split ? keys[lane * a.top + j - 1] : j == 1 ? 0 : ~0ull;
                 if (j == 1) {
-                    g = wave_kth(g, a.top);
+                    first = wave_kth(first, a.top);
                 } else {
                     for (int o = 1; o < 64; o <<= 1) {
-                        const uint64_t y = __shfl_xor((unsigned long long)g, o);
-                        g = std::min(g, y);
+                        const uint64_t y = __shfl_xor((unsigned long long)first, o);
+                        first = std::min(first, y);
                     }
                 }
-                if (threadIdx.x == 0) bound = g;
+                if (threadIdx.x == 0) bound = first;
             }
             __syncthreads();
-            for (int c = threadIdx.x; c < split * a.top; c += kLpBlock) {
-                const uint64_t key = keys[c];
-                if (key && key >= bound) buf[atomicAdd(&count, 1)] = key;
-            }
+#pragma unroll
+            for (int i = 0; i < kKeys; i++)
+                if (key[i] && key[i] >= bound) buf[atomicAdd(&count, 1)] = key[i];
+            for (int c = threadIdx.x + kKeys * kLpBlock; c < split * a.top; c += kLpBlock)
+                if (keys[c] && keys[c] >= bound) buf[atomicAdd(&count, 1)] = keys[c];
             __syncthreads();
-            rank_keys(buf, count, a.top, top);
+            rank_keys<kLpBlock>(buf, count, a.top, top, threadIdx.x);
             __syncthreads();
         }
-        lp_finish(a, r, s, top);
+        lp_finish<kLpBlock>(a, r, s, asked, top, threadIdx.x);
+        if constexpr (TOP) __syncthreads();
     }
 }
 
@@ -330,21 +402,26 @@ int64_t logprobs_part_bytes(const LogProbsArgs &a) {
     return split == 1 ? 0 : a.t * split * (int64_t)(sizeof(LpStat) + 8 * a.top);
 }
 
+template <int TEAM, bool SPLIT> static void logprobs(const LogProbsArgs &a, int split, hipStream_t s) {
+    const unsigned grid = (unsigned)std::min<int64_t>((a.t * split + kLpBlock / TEAM - 1) / (kLpBlock / TEAM), 1 << 20);
+    if (a.top) k_logprobs<TEAM, true, SPLIT><<<grid, kLpBlock, 0, s>>>(a, split);
+    else k_logprobs<TEAM, false, SPLIT><<<grid, kLpBlock, 0, s>>>(a, split);
+}
+
 hipError_t launch_logprobs(const LogProbsArgs &a, hipStream_t s) {
     const int split = lp_split(a);
-    const unsigned grid = (unsigned)std::min<int64_t>(a.t * split, 1 << 20);
-    if (split == 1) {
-        if (a.top) k_logprobs<true, false><<<grid, kLpBlock, 0, s>>>(a, 1);
-        else k_logprobs<false, false><<<grid, kLpBlock, 0, s>>>(a, 1);
-        return hipGetLastError();
+    if (split > 1) {
+        logprobs<kLpBlock, true>(a, split, s);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+        const unsigned rows = (unsigned)std::min<int64_t>(a.t, 1 << 20);
+        if (a.top) k_logprobs_join<true><<<rows, kLpBlock, 0, s>>>(a, split);
+        else k_logprobs_join<false><<<rows, kLpBlock, 0, s>>>(a, split);
+    } else if (a.v <= 4096) {
+        logprobs<64, false>(a, 1, s);
+    } else {
+        logprobs<kLpBlock, false>(a, 1, s);
     }
-    if (a.top) k_logprobs<true, true><<<grid, kLpBlock, 0, s>>>(a, split);
-    else k_logprobs<false, true><<<grid, kLpBlock, 0, s>>>(a, split);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    const unsigned rows = (unsigned)std::min<int64_t>(a.t, 1 << 20);
-    if (a.top) k_logprobs_join<true><<<rows, kLpBlock, 0, s>>>(a, split);
-    else k_logprobs_join<false><<<rows, kLpBlock, 0, s>>>(a, split);
     return hipGetLastError();
 }
 
