@@ -452,6 +452,18 @@ __device__ __forceinline__ void f8_wave_sync() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
+// The tile of a workgroup, false if it has none: tiles in groups of eight rows of them, down a group's columns one after
+// the other, and a contiguous range of that order for each XCD (workgroups go round the 8 XCDs), so that an XCD's cache
+// is asked for few rows of A and of B (64x4096x4096 in tiles of 32x32 8.0 us against 9.8 in the grid's order).
+__device__ __forceinline__ bool f8_tile(int tm, int tn, int *im, int *in) {
+    const int tiles = tm * tn, per = (tiles + 7) / 8, t = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    if ((int)(blockIdx.x >> 3) >= per || t >= tiles) return false;
+    const int group = t / (8 * tn), first = 8 * group, rows = min(tm - first, 8), at = t - group * 8 * tn;
+    *im = first + at % rows;
+    *in = at / rows;
+    return true;
+}
+
 template <int FA, int FB, bool BROWS, int TM, int TN, int WM, int WN, int S, int OCC>
 __global__ __launch_bounds__(64 * WM * WN, OCC) void k_matmul_blocks(MatMulBlocksArgs p, int tm, int tn) {
     constexpr int NW = WM * WN, BM = 32 * TM * WM, BN = 32 * TN * WN, R = BM + BN;
@@ -463,12 +475,9 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void k_matmul_blocks(MatMulBlock
     __shared__ __attribute__((aligned(256))) float sc[S + 1][SCALES];  // a block's scales are read one block later
     const int l = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = l >> 5;
 
-    // tiles in groups of eight rows of tiles, contiguous ranges of them to each XCD (workgroups go round the 8 XCDs)
-    const int tiles = tm * tn, per = (tiles + 7) / 8;
-    const int t = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-    if ((int)(blockIdx.x >> 3) >= per || t >= tiles) return;
-    const int group = t / (8 * tn), first = 8 * group, gs = min(tm - first, 8), in = t - group * 8 * tn;
-    const int m0 = (first + in % gs) * BM, n0 = in / gs * BN;
+    int im0, in0;
+    if (!f8_tile(tm, tn, &im0, &in0)) return;
+    const int m0 = im0 * BM, n0 = in0 * BN;
 
     const int64_t kb = (p.k + 127) / 128;
     const uint8_t *abase = p.a + m0 * p.k, *bbase = p.b + n0 * p.k;
@@ -547,14 +556,15 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void k_matmul_blocks(MatMulBlock
 // from p.m on only reach results that are not stored).  CHUNKS: rows of whole aligned 16-byte chunks, loaded straight to
 // LDS; other rows go through registers, a block ahead too.
 template <int FA, int FB, bool BROWS, int TM, int TN, int LA, int MAXW, bool CHUNKS>
-__global__ __launch_bounds__(64 * MAXW) void k_matmul_blocks_thin(MatMulBlocksArgs p, int tm) {
+__global__ __launch_bounds__(64 * MAXW) void k_matmul_blocks_thin(MatMulBlocksArgs p, int tm, int tn) {
     constexpr int BM = 32 * TM, BN = 32 * TN, LB = BN / 8, L = LA + LB, LS = (BM + BN) / 64;
     constexpr int STAGE = (BM + BN) * 128 + LS * 256;
     __shared__ __attribute__((aligned(1024))) char sm[MAXW * 2 * STAGE];
     const int l = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), W = blockDim.x >> 6, h = l >> 5;
     char *mine = sm + w * 2 * STAGE;
-    // neighbouring workgroups take the row tiles of one range of B's rows
-    const int64_t m0 = (int64_t)(blockIdx.x % tm) * BM, n0 = (int64_t)(blockIdx.x / tm) * BN;
+    int im0, in0;
+    if (!f8_tile(tm, tn, &im0, &in0)) return;
+    const int64_t m0 = (int64_t)im0 * BM, n0 = (int64_t)in0 * BN;
     const int64_t kb = (p.k + 127) / 128;
     const int row_n = BROWS ? 1 : 128;
     const uint8_t *abase = p.a + m0 * p.k, *bbase = p.b + n0 * p.k;
@@ -659,8 +669,9 @@ template <int FA, int FB, bool BROWS, int TM, int TN, int LA, int MAXW>
 static void thin(const MatMulBlocksArgs &p, bool chunks, hipStream_t s) {
     const int64_t tm = (p.m + 32 * TM - 1) / (32 * TM), tn = (p.n + 32 * TN - 1) / (32 * TN);
     const unsigned threads = 64 * (unsigned)std::max<int64_t>(1, std::min<int64_t>(MAXW, (p.k + 127) / 128));
-    if (chunks) k_matmul_blocks_thin<FA, FB, BROWS, TM, TN, LA, MAXW, true><<<(unsigned)(tm * tn), threads, 0, s>>>(p, (int)tm);
-    else k_matmul_blocks_thin<FA, FB, BROWS, TM, TN, LA, MAXW, false><<<(unsigned)(tm * tn), threads, 0, s>>>(p, (int)tm);
+    const unsigned grid = (unsigned)((tm * tn + 7) / 8 * 8);
+    if (chunks) k_matmul_blocks_thin<FA, FB, BROWS, TM, TN, LA, MAXW, true><<<grid, threads, 0, s>>>(p, (int)tm, (int)tn);
+    else k_matmul_blocks_thin<FA, FB, BROWS, TM, TN, LA, MAXW, false><<<grid, threads, 0, s>>>(p, (int)tm, (int)tn);
 }
 
 // The kernel of a product by its tiles of Y, one workgroup each, against the chip's 256 CUs (us on one device, e4m3):

@@ -47,11 +47,11 @@ __device__ __forceinline__ LpStat stat_merge(LpStat a, LpStat b) {
     return {m, a.r + b.r, a.t + b.t, a.n + b.n};
 }
 
+__device__ __forceinline__ LpStat stat_xor(const LpStat &s, int o) {
+    return {__shfl_xor(s.m, o), __shfl_xor(s.r, o), __shfl_xor(s.t, o), __shfl_xor(s.n, o)};
+}
 __device__ __forceinline__ LpStat stat_wave(LpStat s) {
-    for (int o = 1; o < 64; o <<= 1) {
-        const LpStat b = {__shfl_xor(s.m, o), __shfl_xor(s.r, o), __shfl_xor(s.t, o), __shfl_xor(s.n, o)};
-        s = stat_merge(s, b);
-    }
+    for (int o = 1; o < 64; o <<= 1) s = stat_merge(s, stat_xor(s, o));
     return s;
 }
 
@@ -113,7 +113,7 @@ __device__ __forceinline__ void stat_add(LpStat &s, const float4 *f, int units) 
     }
 }
 
-// A row is a team's work: one wave's (TEAM 64, four rows a workgroup) or the whole workgroup's (TEAM 256).
+// A row is a team's work: one wave's (TEAM 64, four rows a workgroup) or a whole workgroup's (TEAM 256 or 1024).
 template <int TEAM> __device__ __forceinline__ void team_sync() {
     if constexpr (TEAM == 64) {
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -158,10 +158,16 @@ __device__ __forceinline__ uint64_t lane_key(uint64_t g, int j) {
 
 // the k-th largest of the wave's keys, distinct but for zeros (none): zero if fewer than k are there
 __device__ __forceinline__ uint64_t wave_kth(uint64_t g, int k) {
+    const uint32_t hi = (uint32_t)(g >> 32);
     int rank = 0;
 #pragma unroll
-    for (int j = 0; j < 64; j++) rank += lane_key(g, j) > g;
-    const uint64_t at = __ballot(g != 0 && rank == k - 1);
+    for (int j = 0; j < 64; j++) rank += (uint32_t)__builtin_amdgcn_readlane((int)hi, j) > hi;
+    uint64_t at = __ballot(hi != 0 && rank == k - 1);
+    if (__popcll(__ballot(rank < k)) != k || __popcll(at) != 1) {  // equal values around the k-th: by unit
+        rank = 0;
+        for (int j = 0; j < 64; j++) rank += lane_key(g, j) > g;
+        at = __ballot(g != 0 && rank == k - 1);
+    }
     return at ? lane_key(g, __builtin_ctzll(at)) : 0;
 }
 // the same of two keys a lane
@@ -187,13 +193,19 @@ __device__ void team_top(const LpRow &row, uint32_t u0, uint32_t u1, int k, uint
     if (lane == 0) sh.count = sh.winners = 0;
     team_sync<TEAM>();
     if (lane < 64) {
-        uint64_t g;
+        uint64_t g = best;
         if constexpr (TEAM == 64) {
-            g = wave_kth(best, k);
-        } else if (k > 32) {  // two keys a lane: 64 of 64 groups would let many logits past the bound
-            g = wave_kth2(std::max(sh.group[lane], sh.group[lane + 64]), std::max(sh.group[lane + 128], sh.group[lane + 192]), k);
+            g = wave_kth(g, k);
         } else {
-            g = wave_kth(std::max(std::max(sh.group[lane], sh.group[lane + 64]), std::max(sh.group[lane + 128], sh.group[lane + 192])), k);
+            uint64_t g2 = 0;
+#pragma unroll
+            for (int w = 0; w < TEAM / 64; w++) {
+                const uint64_t y = sh.group[64 * w + lane];
+                if (w < TEAM / 128) g = std::max(g, y);
+                else g2 = std::max(g2, y);
+            }
+            // over half of the 64 groups would let many logits past the bound: then 128 of them
+            g = k > 32 ? wave_kth2(g, g2, k) : wave_kth(std::max(g, g2), k);
         }
         if (lane == 0) sh.bound = g;
     }
@@ -288,8 +300,8 @@ __device__ __forceinline__ void lp_finish(const LogProbsArgs &a, int64_t row, co
 
 // A part of a row (SPLIT: kLpSplit parts at most, their sums and keys to a.part) or a whole row for each team.
 template <int TEAM, bool TOP, bool SPLIT>
-__global__ __launch_bounds__(kLpBlock) void k_logprobs(LogProbsArgs a, int split) {
-    constexpr int TEAMS = kLpBlock / TEAM;
+__global__ __launch_bounds__(TEAM > kLpBlock ? TEAM : kLpBlock) void k_logprobs(LogProbsArgs a, int split) {
+    constexpr int TEAMS = TEAM > kLpBlock ? 1 : kLpBlock / TEAM;
     __shared__ LpShared<TEAM> shared[TEAMS];
     const int lane = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
     LpShared<TEAM> &sh = shared[team];
@@ -324,7 +336,12 @@ __global__ __launch_bounds__(kLpBlock) void k_logprobs(LogProbsArgs a, int split
             __syncthreads();  // the previous row's use of sh
             if ((threadIdx.x & 63) == 0) sh.wave[threadIdx.x >> 6] = s;
             __syncthreads();
-            s = stat_merge(stat_merge(sh.wave[0], sh.wave[1]), stat_merge(sh.wave[2], sh.wave[3]));
+            if constexpr (TEAM == 256) {
+                s = stat_merge(stat_merge(sh.wave[0], sh.wave[1]), stat_merge(sh.wave[2], sh.wave[3]));
+            } else {
+                s = sh.wave[threadIdx.x & (TEAM / 64 - 1)];
+                for (int o = 1; o < TEAM / 64; o <<= 1) s = stat_merge(s, stat_xor(s, o));
+            }
         }
         if constexpr (TOP)
             team_top<TEAM>(row, u0, u1, a.top, best > -__builtin_inff() ? lp_key(best, best_u) : 0, sh, lane);
@@ -391,10 +408,17 @@ __global__ __launch_bounds__(kLpBlock) void k_logprobs_join(LogProbsArgs a, int 
     }
 }
 
-// Parts of a row: about four workgroups a CU over all rows, parts of at least 2048 logits, at most kLpSplit.
+// How rows are read, by the time of a call (us, top 5 unless said):
+//   up to 4096 logits a wave each (4096x4000 19 against 33 with a workgroup each);
+//   up to 24576, or from 384 rows on, a workgroup of 256 each (64x10000 7.9 against 9.3 with 1024 threads and 10.5 in
+//     parts, 384x30522 16.4 against 22.6 and 20.7, 700x131072 75.6 against 85.0 and 89.1);
+//   few rows of more than 32768 in parts, joined by a second launch: about four workgroups a CU over all rows, parts of at
+//     least 2048 logits (1x131072 top 20 11.5 against 22.8 with 1024 threads, 64x50001 13.6 against 14.2);
+//   the others a workgroup of 1024 each (192x65536 16.6 against 23.3 with 256 and 21.0 in parts, 64x30522 11.3, 12.2, 13.1).
+static int lp_team(const LogProbsArgs &a) { return a.v <= 4096 ? 64 : a.v <= 24576 || a.t >= 384 ? 256 : 1024; }
 static int lp_split(const LogProbsArgs &a) {
-    const int64_t want = (1024 + a.t - 1) / a.t, most = a.v / 2048;
-    return (int)std::max<int64_t>(1, std::min<int64_t>({want, most, kLpSplit}));
+    if (a.v <= 32768 || a.t >= 96) return 1;
+    return (int)std::min<int64_t>({(1024 + a.t - 1) / a.t, a.v / 2048, kLpSplit});
 }
 
 int64_t logprobs_part_bytes(const LogProbsArgs &a) {
@@ -403,24 +427,27 @@ int64_t logprobs_part_bytes(const LogProbsArgs &a) {
 }
 
 template <int TEAM, bool SPLIT> static void logprobs(const LogProbsArgs &a, int split, hipStream_t s) {
-    const unsigned grid = (unsigned)std::min<int64_t>((a.t * split + kLpBlock / TEAM - 1) / (kLpBlock / TEAM), 1 << 20);
-    if (a.top) k_logprobs<TEAM, true, SPLIT><<<grid, kLpBlock, 0, s>>>(a, split);
-    else k_logprobs<TEAM, false, SPLIT><<<grid, kLpBlock, 0, s>>>(a, split);
+    constexpr int block = std::max(TEAM, kLpBlock), teams = block / TEAM;
+    const unsigned grid = (unsigned)std::min<int64_t>((a.t * split + teams - 1) / teams, 1 << 20);
+    if (a.top) k_logprobs<TEAM, true, SPLIT><<<grid, block, 0, s>>>(a, split);
+    else k_logprobs<TEAM, false, SPLIT><<<grid, block, 0, s>>>(a, split);
 }
 
 hipError_t launch_logprobs(const LogProbsArgs &a, hipStream_t s) {
     const int split = lp_split(a);
     if (split > 1) {
-        logprobs<kLpBlock, true>(a, split, s);
+        logprobs<256, true>(a, split, s);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
         const unsigned rows = (unsigned)std::min<int64_t>(a.t, 1 << 20);
         if (a.top) k_logprobs_join<true><<<rows, kLpBlock, 0, s>>>(a, split);
         else k_logprobs_join<false><<<rows, kLpBlock, 0, s>>>(a, split);
-    } else if (a.v <= 4096) {
-        logprobs<64, false>(a, 1, s);
-    } else {
-        logprobs<kLpBlock, false>(a, 1, s);
+        return hipGetLastError();
+    }
+    switch (lp_team(a)) {
+    case 64: logprobs<64, false>(a, 1, s); break;
+    case 256: logprobs<256, false>(a, 1, s); break;
+    default: logprobs<1024, false>(a, 1, s); break;
     }
     return hipGetLastError();
 }
