@@ -3,6 +3,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "lx_device.h"
 #include "lx_kernels.h"
@@ -271,6 +272,20 @@ template <int N> __device__ __forceinline__ void f8_wait_barrier() {
 #endif
 }
 
+// A wave's own waits: all but its last N direct loads, and its LDS operations, are done; nothing that touches memory
+// moves across.
+template <int N> __device__ __forceinline__ void f8_wait() {
+    static_assert(N >= 0 && N < 64, "vmcnt range");
+#if defined(__HIP_DEVICE_COMPILE__)
+    __asm__ volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+#endif
+}
+__device__ __forceinline__ void f8_wait_lds() {
+#if defined(__HIP_DEVICE_COMPILE__)
+    __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#endif
+}
+
 // A block of K for a wave's TM x TN tiles of 32x32 is read in four chunks of 32 codes a row (the lane's 16 bytes of
 // chunk c are k = 32 c + 16 h .. + 15 of its row: the same permutation of k on both sides), and multiplied in eight
 // steps of half a chunk.
@@ -326,10 +341,13 @@ template <bool BROWS, int TM, int TN> struct F8Scales {
 // One block: the block before's products (part) are scaled into acc with the scales at sa, sb, then this block's are
 // computed.  The order keeps the matrix unit fed and is pinned, since the compiler's own puts the LDS reads next to
 // their use: a chunk is read a chunk ahead, and between one matrix instruction and the next stand the conversions of
-// an operand of the next step and, in the first step, the scaling of the tile that is overwritten next.
-template <int FA, int FB, bool BROWS, int TM, int TN, bool LATE>
+// an operand of the next step and, in the first step, the scaling of the tile that is overwritten next.  So do the
+// direct loads of a later block, feed(slot, slots) after each matrix instruction: issued together they hold the wave
+// up for as long as the CU takes to address them (16 cycles each).  LATE false: this block's own products are scaled,
+// after them, and the loads go into the stage just read, in the second half; else into another, in the first.
+template <int FA, int FB, bool BROWS, int TM, int TN, bool LATE, typename F>
 __device__ __forceinline__ void f8_block(const char *ap, const char *bp, const float *sa, const float *sb, int h, int swz,
-                                         f8_v16f (&part)[TN][TM], f8_v16f (&acc)[TN][TM]) {
+                                         f8_v16f (&part)[TN][TM], f8_v16f (&acc)[TN][TM], F &&feed) {
     constexpr int T = TM * TN, P = TM + TN;
     F8Raw<TM, TN> r[2];
     F8Step<TM, TN> s[2];
@@ -343,11 +361,14 @@ __device__ __forceinline__ void f8_block(const char *ap, const char *bp, const f
     if constexpr (LATE) sc.add(part[0][0], acc[0][0], 0, 0);
 #pragma unroll
     for (int t = 0; t < 8; t++) {
+        if (!LATE && t == 4) f8_wait_lds();
 #pragma unroll
         for (int i = 0; i < T; i++) {
             const int in = i / TM, im = i % TM;
             f8_pin();
             part[in][im] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(s[t & 1].b[in], s[t & 1].a[im], t ? part[in][im] : f8_v16f{}, 0, 0, 0);
+            f8_pin();
+            if (LATE ? t < 4 : t >= 4) feed((t & 3) * T + i, 4 * T);
             f8_pin();
             if (i == 0 && (t == 1 || t == 3)) {
                 r[t == 3].read(ap, bp, t == 1 ? 2 : 3, h, swz);
@@ -433,19 +454,6 @@ __device__ __forceinline__ void f8_store(const MatMulBlocksArgs &p, const float 
     }
 }
 
-// A wave's own waits: all but its last N direct loads, and its LDS operations, are done; nothing that touches memory
-// moves across.
-template <int N> __device__ __forceinline__ void f8_wait() {
-    static_assert(N >= 0 && N < 64, "vmcnt range");
-#if defined(__HIP_DEVICE_COMPILE__)
-    __asm__ volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
-#endif
-}
-__device__ __forceinline__ void f8_wait_lds() {
-#if defined(__HIP_DEVICE_COMPILE__)
-    __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-#endif
-}
 __device__ __forceinline__ void f8_wave_sync() {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
@@ -497,23 +505,29 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void k_matmul_blocks(MatMulBlock
         soff[i] = (uint32_t)(row * (int)kb * 4);
     }
     const int tail = (int)(p.k & 127);  // codes of a last block that is not whole
-    auto load = [&](int64_t j, char *st, float *scl) {
-        if (tail && j == kb - 1) {
+    // direct load i of the wave's L + LS of a stage (none of a cut last block's)
+    auto load_one = [&](int i, int64_t j, char *st, float *scl) {
+        if (i < L) f8_load_lds16((NW * i < BM / 8 ? abase : bbase) + 128 * j, off[i], st + 1024 * (w + NW * i));
+        else f8_load_lds4((64 * (w + NW * (i - L)) < BM ? sabase : sbbase) + j, soff[i - L], scl + 64 * (w + NW * (i - L)));
+    };
+    auto load_cut = [&](int64_t j, char *st, float *scl) {
 #pragma unroll
-            for (int i = 0; i < L; i++) {
-                const int r = 8 * (w + NW * i) + (l >> 3), c = (l & 7) ^ ((r >> 1) & 7);
-                char *lds = st + 1024 * (w + NW * i);
-                if (16 * c < tail) f8_load_lds16((NW * i < BM / 8 ? abase : bbase) + 128 * j, off[i], lds);
-                else *(uint4 *)(lds + 16 * l) = uint4{0, 0, 0, 0};
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < L; i++)
-                f8_load_lds16((NW * i < BM / 8 ? abase : bbase) + 128 * j, off[i], st + 1024 * (w + NW * i));
+        for (int i = 0; i < L; i++) {
+            const int r = 8 * (w + NW * i) + (l >> 3), c = (l & 7) ^ ((r >> 1) & 7);
+            char *lds = st + 1024 * (w + NW * i);
+            if (16 * c < tail) load_one(i, j, st, scl);
+            else *(uint4 *)(lds + 16 * l) = uint4{0, 0, 0, 0};
         }
 #pragma unroll
-        for (int i = 0; i < LS; i++)
-            f8_load_lds4((64 * (w + NW * i) < BM ? sabase : sbbase) + j, soff[i], scl + 64 * (w + NW * i));
+        for (int i = L; i < L + LS; i++) load_one(i, j, st, scl);
+    };
+    auto load = [&](int64_t j, char *st, float *scl) {
+        if (tail && j == kb - 1) {
+            load_cut(j, st, scl);
+        } else {
+#pragma unroll
+            for (int i = 0; i < L + LS; i++) load_one(i, j, st, scl);
+        }
     };
 
     f8_v16f acc[TN][TM] = {}, part[TN][TM] = {};
@@ -523,19 +537,34 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void k_matmul_blocks(MatMulBlock
     for (int s = 0; s < S - 1; s++)
         if (s < kb) load(s, sm[s], sc[s]);
     int cur = 0, scur = 0;
-    for (int64_t j = 0; j < kb; j++) {
+    // block j; FEED: block j + S - 1 is there and whole
+    auto step = [&](int64_t j, auto feed_) {
+        constexpr bool FEED = decltype(feed_)::value;
         // the last S - 2 stages ahead may still be landing; near the end there are fewer
-        if (S > 2 && j + S - 2 < kb) f8_wait_barrier<(S - 2) * (L + LS)>();
+        if (S > 2 && (FEED || j + S - 2 < kb)) f8_wait_barrier<(S - 2) * (L + LS)>();
         else f8_wait_barrier<0>();
         const char *st = sm[cur], *ap = st + (wm * TM * 32 + (l & 31)) * 128, *bp = st + (BM + wn * TN * 32 + (l & 31)) * 128;
         const int before = scur == 0 ? S : scur - 1;  // the block before's scales
-        int ahead = scur + S - 1;
-        if (j + S - 1 < kb) load(j + S - 1, sm[cur == 0 ? S - 1 : cur - 1], sc[ahead > S ? ahead - S - 1 : ahead]);
+        const int ahead = scur + S - 1;
+        const int64_t jn = j + S - 1;
+        char *stn = sm[cur == 0 ? S - 1 : cur - 1];
+        float *scn = sc[ahead > S ? ahead - S - 1 : ahead];
+        if (!FEED && jn == kb - 1) load_cut(jn, stn, scn);
         cur = cur + 1 == S ? 0 : cur + 1;
         scur = scur == S ? 0 : scur + 1;
         const float *c = sc[before];
-        f8_block<FA, FB, BROWS, TM, TN, true>(ap, bp, c + wm * TM * 32 + (l & 31), c + BM + wn * TN * 32, h, swz, part, acc);
-    }
+        f8_block<FA, FB, BROWS, TM, TN, true>(ap, bp, c + wm * TM * 32 + (l & 31), c + BM + wn * TN * 32, h, swz, part, acc,
+                                              [&](int slot, int slots) {
+            if constexpr (FEED) {
+#pragma unroll
+                for (int i = slot * (L + LS) / slots; i < (slot + 1) * (L + LS) / slots; i++) load_one(i, jn, stn, scn);
+            }
+        });
+    };
+    const int64_t fed = kb - (S - 1) - (tail ? 1 : 0);
+    int64_t j = 0;
+    for (; j < fed; j++) step(j, std::true_type());
+    for (; j < kb; j++) step(j, std::false_type());
     if (kb) {
         const float *c = sc[scur == 0 ? S : scur - 1];
         f8_scale_add<BROWS>(part, c + wm * TM * 32 + (l & 31), c + BM + wn * TN * 32, h, acc);
@@ -583,33 +612,36 @@ __global__ __launch_bounds__(64 * MAXW) void k_matmul_blocks_thin(MatMulBlocksAr
         const int r = 64 * i + l;
         soff[i] = (uint32_t)((r < BM ? min(r, rows_a) : min(r - BM, rows_b) / row_n) * (int)kb * 4);
     }
-    auto scales = [&](int64_t j, char *st) {
-#pragma unroll
-        for (int i = 0; i < LS; i++) {
-            if constexpr (BM % 64 == 0) {
-                f8_load_lds4((64 * i < BM ? sabase : sbbase) + j, soff[i], st + (BM + BN) * 128 + 256 * i);
-            } else {  // the first half of the lanes A's rows, the second B's
-                if (l < BM) f8_load_lds4(sabase + j, soff[i], st + (BM + BN) * 128);
-                else f8_load_lds4(sbbase + j, soff[i], st + (BM + BN) * 128);
-            }
+    auto scales = [&](int64_t j, char *st, int i) {
+        if constexpr (BM % 64 == 0) {
+            f8_load_lds4((64 * i < BM ? sabase : sbbase) + j, soff[i], st + (BM + BN) * 128 + 256 * i);
+        } else {  // the first half of the lanes A's rows, the second B's
+            if (l < BM) f8_load_lds4(sabase + j, soff[i], st + (BM + BN) * 128);
+            else f8_load_lds4(sbbase + j, soff[i], st + (BM + BN) * 128);
         }
     };
     constexpr int NL = L + (BM % 64 == 0 ? LS : 2);  // direct loads a stage
-    auto load = [&](int64_t j, char *st) {
-        const bool cut = tail && j == kb - 1;
+    auto load_one = [&](int i, int64_t j, char *st) {  // i-th of L + LS (none of a cut last block's)
+        if (i < L) f8_load_lds16((i < LA ? abase : bbase) + 128 * j, off[i], st + 1024 * (i < LA ? i : i - LA + BM / 8));
+        else scales(j, st, i - L);
+    };
+    auto load_cut = [&](int64_t j, char *st) {
 #pragma unroll
         for (int i = 0; i < L; i++) {
-            const int g = i < LA ? i : i - LA + BM / 8;
-            const uint8_t *base = (i < LA ? abase : bbase) + 128 * j;
-            if (!cut) {
-                f8_load_lds16(base, off[i], st + 1024 * g);
-            } else {
-                const int r = 8 * g + (l >> 3), c = (l & 7) ^ ((r >> 1) & 7);
-                if (16 * c < tail) f8_load_lds16(base, off[i], st + 1024 * g);
-                else *(uint4 *)(st + 1024 * g + 16 * l) = uint4{0, 0, 0, 0};
-            }
+            const int g = i < LA ? i : i - LA + BM / 8, r = 8 * g + (l >> 3), c = (l & 7) ^ ((r >> 1) & 7);
+            if (16 * c < tail) load_one(i, j, st);
+            else *(uint4 *)(st + 1024 * g + 16 * l) = uint4{0, 0, 0, 0};
         }
-        scales(j, st);
+#pragma unroll
+        for (int i = L; i < L + LS; i++) load_one(i, j, st);
+    };
+    auto load = [&](int64_t j, char *st) {
+        if (tail && j == kb - 1) {
+            load_cut(j, st);
+        } else {
+#pragma unroll
+            for (int i = 0; i < L + LS; i++) load_one(i, j, st);
+        }
     };
     uint4 reg[CHUNKS ? 1 : L];
     auto fetch = [&](int64_t j) {
@@ -630,32 +662,43 @@ __global__ __launch_bounds__(64 * MAXW) void k_matmul_blocks_thin(MatMulBlocksAr
 
     f8_v16f acc[TN][TM] = {}, part[TN][TM];
     const int swz = ((l & 31) >> 1) & 7;
-    auto block = [&](const char *st) {
+    auto block = [&](const char *st, auto &&feed) {
         const float *sc = (const float *)(st + (BM + BN) * 128);
-        f8_block<FA, FB, BROWS, TM, TN, false>(st + (l & 31) * 128, st + (BM + (l & 31)) * 128, sc + (l & 31), sc + BM, h, swz, part, acc);
+        f8_block<FA, FB, BROWS, TM, TN, false>(st + (l & 31) * 128, st + (BM + (l & 31)) * 128, sc + (l & 31), sc + BM, h, swz, part, acc,
+                                                 feed);
     };
     if constexpr (CHUNKS) {
         if (w < kb) load(w, mine);
         if (w + W < kb) load(w + W, mine + STAGE);
         int cur = 0;
-        for (int64_t j = w; j < kb; j += W) {
+        auto step = [&](int64_t j, auto feed_) {
+            constexpr bool FEED = decltype(feed_)::value;  // block j + 2 W is there and whole
             char *st = mine + cur * STAGE;
-            if (j + W < kb) f8_wait<NL>();
+            if (FEED || j + W < kb) f8_wait<NL>();
             else f8_wait<0>();
-            block(st);
-            f8_wait_lds();  // this stage has been read
-            if (j + 2 * W < kb) load(j + 2 * W, st);
+            block(st, [&](int slot, int slots) {
+                if constexpr (FEED) {
+#pragma unroll
+                    for (int i = slot * (L + LS) / slots; i < (slot + 1) * (L + LS) / slots; i++) load_one(i, j + 2 * W, st);
+                }
+            });
+            if (!FEED && j + 2 * W == kb - 1) load_cut(j + 2 * W, st);
             cur ^= 1;
-        }
+        };
+        const int64_t fed = kb - 2 * W - (tail ? 1 : 0);
+        int64_t j = w;
+        for (; j < fed; j += W) step(j, std::true_type());
+        for (; j < kb; j += W) step(j, std::false_type());
     } else {
         if (w < kb) fetch(w);
         for (int64_t j = w; j < kb; j += W) {
             f8_wait_lds();
             drop(j, mine);
-            scales(j, mine);
+#pragma unroll
+            for (int i = 0; i < LS; i++) scales(j, mine, i);
             if (j + W < kb) fetch(j + W);
             f8_wait<0>();
-            block(mine);
+            block(mine, [](int, int) {});
         }
     }
     // every wave's sums in its own stage, joined in the waves' order
