@@ -423,9 +423,9 @@ __device__ __forceinline__ void f8_put(float *t, const f8_v16f (&acc)[TN][TM], i
 }
 
 // Writes rows [0, rows) of such a tile, summed over `parts` of them `stride` floats apart in order, to y's rows from
-// (m0, n0) on, plus the bias: whole rows of neighbouring floats by neighbouring threads.
-template <int TM, int TN>
-__device__ __forceinline__ void f8_store(const MatMulBlocksArgs &p, const float *t, int parts, int stride, int64_t m0, int64_t n0,
+// (m0, n0) on, plus the bias: whole rows of neighbouring floats by neighbouring threads.  PAST: past the caches.
+template <int TM, int TN, bool PAST>
+__device__ __forceinline__ void f8_store_rows(const MatMulBlocksArgs &p, const float *t, int parts, int stride, int64_t m0, int64_t n0,
                                          int thread, int threads) {
     constexpr int W = 32 * TN;
     const int rows = (int)std::min<int64_t>(32 * TM, p.m - m0), cols = (int)std::min<int64_t>(W, p.n - n0);
@@ -440,7 +440,8 @@ __device__ __forceinline__ void f8_store(const MatMulBlocksArgs &p, const float 
             for (int k = 1; k < parts; k++) v += *(const f8_v4f *)(f + k * stride);
             if (bias)
                 for (int e = 0; e < 4; e++) v[e] += bias[4 * s + e];
-            *(f8_v4f *)(y + m * p.n + 4 * s) = v;
+            if constexpr (PAST) __builtin_nontemporal_store(v, (f8_v4f *)(y + m * p.n + 4 * s));
+            else *(f8_v4f *)(y + m * p.n + 4 * s) = v;
         }
     } else {
         for (int i = thread; i < rows * W; i += threads) {
@@ -449,7 +450,9 @@ __device__ __forceinline__ void f8_store(const MatMulBlocksArgs &p, const float 
             const float *f = t + m * W + 4 * ((n / 4) ^ f8_turn<TN>(m)) + n % 4;
             float v = *f;
             for (int k = 1; k < parts; k++) v += f[k * stride];
-            y[m * p.n + n] = bias ? v + bias[n] : v;
+            if (bias) v += bias[n];
+            if constexpr (PAST) __builtin_nontemporal_store(v, y + m * p.n + n);
+            else y[m * p.n + n] = v;
         }
     }
 }
@@ -458,6 +461,16 @@ __device__ __forceinline__ void f8_wave_sync() {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// Results of more than the L2s hold (32 MB) go past them: 8192x4096x8192 495 us against 479, and a vocabulary's logits,
+// [512, 30522], leave the inputs of the next call there (the product alone 38.0 against 39.1, with the quantisation
+// before it and the log-probabilities after it 66.5 against 64.5).
+template <int TM, int TN>
+__device__ __forceinline__ void f8_store(const MatMulBlocksArgs &p, const float *t, int parts, int stride, int64_t m0, int64_t n0,
+                                         int thread, int threads) {
+    if (p.m * p.n > (8 << 20)) f8_store_rows<TM, TN, true>(p, t, parts, stride, m0, n0, thread, threads);
+    else f8_store_rows<TM, TN, false>(p, t, parts, stride, m0, n0, thread, threads);
 }
 
 // The tile of a workgroup, false if it has none: tiles in groups of eight rows of them, down a group's columns one after
@@ -721,8 +734,8 @@ static void thin(const MatMulBlocksArgs &p, bool chunks, hipStream_t s) {
 //   128x128 from 256 of them on: [512,768]x[30522,768] 39 against 48 in tiles of 64x64, 8192x4096x8192 492 against 640;
 //     4096x768x768, 192 of them, 13.0 against 12.5
 //   64x64 from 257 on: 2048x1024x1024 11.4 against 12.9 with waves over K; 1024x1024x1024, 256 of them, 8.6 against 7.5
-//   64x64 with waves over K from 128 on, and for rows that are not whole chunks: 788x768x768 6.9 against 7.4 in tiles
-//     of 32x32; 333x1232x1001, 96 of them, 12.1 against 7.8
+//   64x64 with waves over K from 129 on, and for rows that are not whole chunks: 788x768x768 6.7 against 7.2 in tiles
+//     of 32x32; 128x4096x4096, 128 of them, 13.1 against 11.5
 //   32x32 with waves over K: eight waves up to 256 of them (64x4096x4096 9.6 against 10.0), more with four, two
 //     workgroups a CU (788x768x768 7.4 against 8.9); of at most eight rows only those of A are read.
 template <int FA, int FB, bool BROWS> static hipError_t matmul_blocks(const MatMulBlocksArgs &p, hipStream_t s) {
@@ -734,7 +747,7 @@ template <int FA, int FB, bool BROWS> static hipError_t matmul_blocks(const MatM
     } else if (chunks && p.m > 32 && tiles(64) > 256) {
         k_matmul_blocks<FA, FB, BROWS, 1, 1, 2, 2, 3, 3>
             <<<(unsigned)((tiles(64) + 7) / 8 * 8), 256, 0, s>>>(p, (int)((p.m + 63) / 64), (int)((p.n + 63) / 64));
-    } else if (p.m > 32 && tiles(64) >= 128) {
+    } else if (p.m > 32 && tiles(64) > 128) {
         thin<FA, FB, BROWS, 2, 2, 8, 4>(p, chunks, s);
     } else if (tiles(32) <= 256) {
         if (p.m <= 8) thin<FA, FB, BROWS, 1, 1, 1, 8>(p, chunks, s);

@@ -129,7 +129,8 @@ SHAPES = [(1, 1, 1), (1, 128, 128), (1, 384, 384), (2, 129, 33), (7, 127, 130), 
           (65, 2048, 100), (1, 4096, 515), (16, 16, 16), (100, 1111, 77), (129, 768, 384), (128, 144, 1000), (257, 400, 300),
           (300, 384, 513), (1000, 272, 129), (512, 1536, 640), (1, 20000, 5),
           (3, 256, 8300), (3, 77, 8300), (200, 333, 1500), (500, 384, 1030), (500, 301, 1030), (1040, 400, 1030), (1088, 256, 1088),
-          (2000, 272, 2100), (2049, 128, 2051), (2000, 131, 2100), (2048, 640, 2048)]
+          (2000, 272, 2100), (2049, 128, 2051), (2000, 131, 2100), (2048, 640, 2048),
+          (4100, 128, 2060), (4100, 144, 2063)]  # results past the caches
 
 
 @pytest.mark.parametrize("m,k,n", SHAPES)
