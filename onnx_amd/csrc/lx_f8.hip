@@ -76,39 +76,47 @@ __device__ __forceinline__ float f8_finite_abs(float x) {
     return a < __builtin_inff() ? a : 0.0f;  // NaN compares false
 }
 
-// Blocks of one row: 32 lanes a block, four values a lane.
-template <int FMT, bool VEC>
+// Blocks of one row: 32 lanes a block, four values a lane, U blocks at once (their loads and reductions overlap).
+template <int FMT, bool VEC, int U>
 __global__ __launch_bounds__(256) void k_quantize_rows(const float *__restrict__ x, uint8_t *__restrict__ q,
-                                                       float *__restrict__ s, int64_t k, int64_t kb, int64_t blocks) {
+                                                       float *__restrict__ s, int64_t k, FastDiv kb, uint32_t blocks) {
     const int lane = threadIdx.x & 31;
-    const int64_t step = (int64_t)gridDim.x * 8;
-    for (int64_t b = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); b < blocks; b += step) {
-        const int64_t row = b / kb, j = b - row * kb;
-        const int64_t base = row * k + j * 128;
-        const int n = (int)std::min<int64_t>(128, k - j * 128);
-        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    const uint32_t b0 = (blockIdx.x * 8 + (threadIdx.x >> 5)) * U;
+    int64_t base[U];
+    int n[U];
+    float v[U][4];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const uint32_t row = fdiv(b0 + u, kb), j = b0 + u - row * kb.d;
+        base[u] = row * k + j * 128;
+        n[u] = b0 + u < blocks ? (int)std::min<int64_t>(128, k - (int64_t)j * 128) : 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[u][i] = 0.0f;
         if constexpr (VEC) {
-            if (4 * lane < n) {
-                const f8_v4f t = *(const f8_v4f *)(x + base + 4 * lane);
-                for (int i = 0; i < 4; i++) v[i] = t[i];
+            if (4 * lane < n[u]) {
+                const f8_v4f t = *(const f8_v4f *)(x + base[u] + 4 * lane);
+                for (int i = 0; i < 4; i++) v[u][i] = t[i];
             }
         } else {
             for (int i = 0; i < 4; i++)
-                if (lane + 32 * i < n) v[i] = x[base + lane + 32 * i];
+                if (lane + 32 * i < n[u]) v[u][i] = x[base[u] + lane + 32 * i];
         }
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
         float m = 0.0f;
-        for (int i = 0; i < 4; i++) m = fmaxf(m, f8_finite_abs(v[i]));
-        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 32));
+        for (int i = 0; i < 4; i++) m = fmaxf(m, f8_finite_abs(v[u][i]));
+        m = group_reduce<32>(m, [](float a, float b) { return fmaxf(a, b); });
         const F8Scale c = f8_scale<FMT>(m);
-        int w = f8_pack2<FMT>(f8_quotient(v[0], c), f8_quotient(v[1], c), 0, false);
-        w = f8_pack2<FMT>(f8_quotient(v[2], c), f8_quotient(v[3], c), w, true);
+        int w = f8_pack2<FMT>(f8_quotient(v[u][0], c), f8_quotient(v[u][1], c), 0, false);
+        w = f8_pack2<FMT>(f8_quotient(v[u][2], c), f8_quotient(v[u][3], c), w, true);
         if constexpr (VEC) {
-            if (4 * lane < n) *(int *)(q + base + 4 * lane) = w;
+            if (4 * lane < n[u]) *(int *)(q + base[u] + 4 * lane) = w;
         } else {
             for (int i = 0; i < 4; i++)
-                if (lane + 32 * i < n) q[base + lane + 32 * i] = (uint8_t)(w >> (8 * i));
+                if (lane + 32 * i < n[u]) q[base[u] + lane + 32 * i] = (uint8_t)(w >> (8 * i));
         }
-        if (lane == 0) s[b] = c.s;
+        if (lane == 0 && n[u]) s[b0 + u] = c.s;
     }
 }
 
@@ -142,7 +150,7 @@ __global__ __launch_bounds__(256) void k_quantize_tiles(const float *__restrict_
             }
             for (int i = 0; i < 4; i++) m = fmaxf(m, f8_finite_abs(v[p][i]));
         }
-        for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+        m = wave_reduce_dpp(m, [](float a, float b) { return fmaxf(a, b); });
         __syncthreads();  // the previous block's reads of part
         if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = m;
         __syncthreads();
@@ -170,10 +178,24 @@ template <int FMT> static hipError_t quantize(const QuantizeArgs &a, hipStream_t
     // four values a lane need rows of whole float4s; others go value by value, 32 neighbours at a time
     const bool vec = a.k % 4 == 0 && ((uintptr_t)a.x & 15) == 0 && ((uintptr_t)a.q & 3) == 0;
     if (a.block_rows == 1) {
-        const int64_t blocks = a.mats * a.rows * kb;
-        const int64_t grid = std::min<int64_t>((blocks + 7) / 8, 1 << 20);
-        if (vec) k_quantize_rows<FMT, true><<<(unsigned)grid, 256, 0, st>>>(a.x, a.q, a.s, a.k, kb, blocks);
-        else k_quantize_rows<FMT, false><<<(unsigned)grid, 256, 0, st>>>(a.x, a.q, a.s, a.k, kb, blocks);
+        // in row ranges of fewer than 2^31 blocks
+        const int64_t rows = a.mats * a.rows, most = std::max<int64_t>(1, ((int64_t)1 << 30) / kb);
+        for (int64_t r = 0; r < rows; r += most) {
+            const uint32_t blocks = (uint32_t)(std::min(most, rows - r) * kb);
+            const float *x = a.x + r * a.k;
+            uint8_t *q = a.q + r * a.k;
+            float *s = a.s + r * kb;
+            const FastDiv d = make_fastdiv((uint32_t)kb);
+            const unsigned g4 = (blocks + 31) / 32, g1 = (blocks + 7) / 8;
+            // four blocks at once where that still gives every CU a workgroup
+            if (g4 >= 256) {
+                if (vec) k_quantize_rows<FMT, true, 4><<<g4, 256, 0, st>>>(x, q, s, a.k, d, blocks);
+                else k_quantize_rows<FMT, false, 4><<<g4, 256, 0, st>>>(x, q, s, a.k, d, blocks);
+            } else {
+                if (vec) k_quantize_rows<FMT, true, 1><<<g1, 256, 0, st>>>(x, q, s, a.k, d, blocks);
+                else k_quantize_rows<FMT, false, 1><<<g1, 256, 0, st>>>(x, q, s, a.k, d, blocks);
+            }
+        }
     } else {
         const int64_t rb = (a.rows + 127) / 128, blocks = a.mats * rb * kb;
         const int64_t grid = std::min<int64_t>(blocks, 1 << 20);
