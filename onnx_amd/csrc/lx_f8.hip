@@ -120,22 +120,26 @@ __global__ __launch_bounds__(256) void k_quantize_rows(const float *__restrict__
     }
 }
 
-// Blocks of 128 rows: one workgroup a block, the values in registers between the maximum and the codes.
+// Blocks of 128 rows: one workgroup a block, the values in registers between the maximum and the codes.  512 threads
+// ([30522, 768] 26.6 us, 4.4 TB/s, and [512, 768] 5.2) keep more of a CU's loads in flight than 1024 (33.7, 5.3) and
+// reach the maximum sooner than 256 (28.5, 6.8).
+constexpr int kTileThreads = 512;
 template <int FMT, bool VEC>
-__global__ __launch_bounds__(256) void k_quantize_tiles(const float *__restrict__ x, uint8_t *__restrict__ q,
+__global__ __launch_bounds__(kTileThreads) void k_quantize_tiles(const float *__restrict__ x, uint8_t *__restrict__ q,
                                                         float *__restrict__ s, int64_t rows, int64_t k, int64_t rb,
                                                         int64_t kb, int64_t blocks) {
-    __shared__ float part[4];
+    constexpr int P = 4096 / kTileThreads, ROWS = kTileThreads / 32;
+    __shared__ float part[kTileThreads / 64];
     const int lane = threadIdx.x & 31, sub = threadIdx.x >> 5;
     for (int64_t b = blockIdx.x; b < blocks; b += gridDim.x) {
         const int64_t mat = b / (rb * kb), in = b - mat * rb * kb, i0 = in / kb, j = in - i0 * kb;
         const int64_t base = (mat * rows + i0 * 128) * k + j * 128;
         const int nr = (int)std::min<int64_t>(128, rows - i0 * 128), n = (int)std::min<int64_t>(128, k - j * 128);
-        float v[16][4];
+        float v[P][4];
         float m = 0.0f;
 #pragma unroll
-        for (int p = 0; p < 16; p++) {
-            const int r = sub + 8 * p;
+        for (int p = 0; p < P; p++) {
+            const int r = sub + ROWS * p;
             for (int i = 0; i < 4; i++) v[p][i] = 0.0f;
             if (r < nr) {
                 if constexpr (VEC) {
@@ -154,11 +158,13 @@ __global__ __launch_bounds__(256) void k_quantize_tiles(const float *__restrict_
         __syncthreads();  // the previous block's reads of part
         if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = m;
         __syncthreads();
-        m = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+        m = part[0];
+#pragma unroll
+        for (int w = 1; w < kTileThreads / 64; w++) m = fmaxf(m, part[w]);
         const F8Scale c = f8_scale<FMT>(m);
 #pragma unroll
-        for (int p = 0; p < 16; p++) {
-            const int r = sub + 8 * p;
+        for (int p = 0; p < P; p++) {
+            const int r = sub + ROWS * p;
             if (r >= nr) continue;
             int w = f8_pack2<FMT>(f8_quotient(v[p][0], c), f8_quotient(v[p][1], c), 0, false);
             w = f8_pack2<FMT>(f8_quotient(v[p][2], c), f8_quotient(v[p][3], c), w, true);
@@ -199,8 +205,8 @@ template <int FMT> static hipError_t quantize(const QuantizeArgs &a, hipStream_t
     } else {
         const int64_t rb = (a.rows + 127) / 128, blocks = a.mats * rb * kb;
         const int64_t grid = std::min<int64_t>(blocks, 1 << 20);
-        if (vec) k_quantize_tiles<FMT, true><<<(unsigned)grid, 256, 0, st>>>(a.x, a.q, a.s, a.rows, a.k, rb, kb, blocks);
-        else k_quantize_tiles<FMT, false><<<(unsigned)grid, 256, 0, st>>>(a.x, a.q, a.s, a.rows, a.k, rb, kb, blocks);
+        if (vec) k_quantize_tiles<FMT, true><<<(unsigned)grid, kTileThreads, 0, st>>>(a.x, a.q, a.s, a.rows, a.k, rb, kb, blocks);
+        else k_quantize_tiles<FMT, false><<<(unsigned)grid, kTileThreads, 0, st>>>(a.x, a.q, a.s, a.rows, a.k, rb, kb, blocks);
     }
     return hipGetLastError();
 }
