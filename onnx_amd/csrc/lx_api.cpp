@@ -2546,6 +2546,18 @@ int check_apart(const lx_tensor *out, const char *oname, const lx_tensor *in, co
 
 int64_t blocks128(int64_t n) { return (n + 127) / 128; }
 
+// Scratch of one call (null for none): the graph's own where the stream is being captured.
+int scratch_for(int64_t bytes, void **p, bool *capturing) {
+    *p = nullptr;
+    *capturing = false;
+    if (!bytes) return LX_OK;
+    hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
+    HIPCHECK(hipStreamIsCapturing(g.stream, &cs), "hipStreamIsCapturing");
+    *capturing = cs != hipStreamCaptureStatusNone;
+    HIPCHECK(alloc_temp(p, bytes, *capturing), "device allocation (temporary)");
+    return LX_OK;
+}
+
 // Outputs this call allocated go back to the pool when it fails after all.
 struct OutputGuard {
     lx_tensor *t;
@@ -2667,7 +2679,11 @@ extern "C" int lx_MatMulBlocks(const lx_tensor *A, const lx_tensor *a_scale, con
         p.fmt_a = A->dtype;
         p.fmt_b = B->dtype;
         p.b_rows = rows ? 1 : 128;
-        HIPCHECK(launch_matmul_blocks(p, g.stream), "MatMulBlocks");
+        bool capturing;
+        if ((st = scratch_for(matmul_blocks_part_bytes(p), &p.part, &capturing))) return st;
+        const hipError_t e = launch_matmul_blocks(p, g.stream);
+        release_temp(p.part, capturing);
+        if (e != hipSuccess) return hip_fail(e, "MatMulBlocks");
     }
     gy.keep = true;
     return LX_OK;
@@ -2738,11 +2754,8 @@ extern "C" int lx_TokenLogProbs(const lx_tensor *logits, const lx_tensor *ids, i
         a.t = t;
         a.v = v;
         a.top = (int32_t)top;
-        hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
-        (void)hipStreamIsCapturing(g.stream, &cs);
-        const bool capturing = cs != hipStreamCaptureStatusNone;
-        const int64_t bytes = logprobs_part_bytes(a);
-        if (bytes) HIPCHECK(alloc_temp(&a.part, bytes, capturing), "device allocation (temporary)");
+        bool capturing;
+        if ((st = scratch_for(logprobs_part_bytes(a), &a.part, &capturing))) return st;
         const hipError_t e = launch_logprobs(a, g.stream);
         release_temp(a.part, capturing);
         if (e != hipSuccess) return hip_fail(e, "TokenLogProbs");

@@ -758,6 +758,26 @@ static void thin(const MatMulBlocksArgs &p, bool chunks, hipStream_t s) {
     else k_matmul_blocks_thin<FA, FB, BROWS, TM, TN, LA, MAXW, false><<<grid, threads, 0, s>>>(p, (int)tm, (int)tn);
 }
 
+// Rows of whole aligned 16-byte chunks: what the direct-to-LDS loads take.
+static bool whole_chunks(const MatMulBlocksArgs &p) { return p.k % 16 == 0 && (((uintptr_t)p.a | (uintptr_t)p.b) & 15) == 0; }
+static int64_t tiles(const MatMulBlocksArgs &p, int64_t b) { return (p.m + b - 1) / b * ((p.n + b - 1) / b); }
+
+// Other rows copied to such, zeros behind them: 16 bytes a thread, A's rows and then B's.
+__global__ __launch_bounds__(256) void k_matmul_blocks_rows(MatMulBlocksArgs p, uint4 *out, FastDiv chunks, uint32_t total) {
+    const uint32_t i = blockIdx.x * 256 + threadIdx.x;
+    if (i >= total) return;
+    const uint32_t r = fdiv(i, chunks), c = 16 * (i - r * chunks.d);
+    const uint8_t *row = r < p.m ? p.a + (int64_t)r * p.k : p.b + (int64_t)(r - p.m) * p.k;
+    out[i] = f8_tail16(f8_load16(row, (int)c, (int)p.k), (int)c, (int)p.k);
+}
+
+// Products of many tiles are worth that copy: (m + n) k bytes read and written against kernels that wait for
+// their loads.
+int64_t matmul_blocks_part_bytes(const MatMulBlocksArgs &p) {
+    const int64_t bytes = (p.m + p.n) * ((p.k + 15) / 16 * 16);
+    return !whole_chunks(p) && p.k > 0 && p.m > 32 && tiles(p, 64) > 256 && bytes / 16 < ((int64_t)1 << 31) ? bytes : 0;
+}
+
 // The kernel of a product by its tiles of Y, one workgroup each, against the chip's 256 CUs (us on one device, e4m3):
 //   128x128 from 256 of them on: [512,768]x[30522,768] 39 against 48 in tiles of 64x64, 8192x4096x8192 492 against 640;
 //     4096x768x768, 192 of them, 13.0 against 12.5
@@ -767,17 +787,16 @@ static void thin(const MatMulBlocksArgs &p, bool chunks, hipStream_t s) {
 //   32x32 with waves over K: eight waves up to 256 of them (64x4096x4096 9.6 against 10.0), more with four, two
 //     workgroups a CU (788x768x768 7.4 against 8.9); of at most eight rows only those of A are read.
 template <int FA, int FB, bool BROWS> static hipError_t matmul_blocks(const MatMulBlocksArgs &p, hipStream_t s) {
-    const bool chunks = p.k % 16 == 0 && (((uintptr_t)p.a | (uintptr_t)p.b) & 15) == 0;
-    auto tiles = [&](int64_t b) { return (p.m + b - 1) / b * ((p.n + b - 1) / b); };
-    if (chunks && tiles(128) >= 256) {
+    const bool chunks = whole_chunks(p);
+    if (chunks && tiles(p, 128) >= 256) {
         k_matmul_blocks<FA, FB, BROWS, 2, 2, 2, 2, 2, 2>
-            <<<(unsigned)((tiles(128) + 7) / 8 * 8), 256, 0, s>>>(p, (int)((p.m + 127) / 128), (int)((p.n + 127) / 128));
-    } else if (chunks && p.m > 32 && tiles(64) > 256) {
+            <<<(unsigned)((tiles(p, 128) + 7) / 8 * 8), 256, 0, s>>>(p, (int)((p.m + 127) / 128), (int)((p.n + 127) / 128));
+    } else if (chunks && p.m > 32 && tiles(p, 64) > 256) {
         k_matmul_blocks<FA, FB, BROWS, 1, 1, 2, 2, 3, 3>
-            <<<(unsigned)((tiles(64) + 7) / 8 * 8), 256, 0, s>>>(p, (int)((p.m + 63) / 64), (int)((p.n + 63) / 64));
-    } else if (p.m > 32 && tiles(64) > 128) {
+            <<<(unsigned)((tiles(p, 64) + 7) / 8 * 8), 256, 0, s>>>(p, (int)((p.m + 63) / 64), (int)((p.n + 63) / 64));
+    } else if (p.m > 32 && tiles(p, 64) > 128) {
         thin<FA, FB, BROWS, 2, 2, 8, 4>(p, chunks, s);
-    } else if (tiles(32) <= 256) {
+    } else if (tiles(p, 32) <= 256) {
         if (p.m <= 8) thin<FA, FB, BROWS, 1, 1, 1, 8>(p, chunks, s);
         else thin<FA, FB, BROWS, 1, 1, 4, 8>(p, chunks, s);
     } else {
@@ -791,7 +810,17 @@ template <int FA, int FB> static hipError_t matmul_blocks(const MatMulBlocksArgs
     return p.b_rows == 1 ? matmul_blocks<FA, FB, true>(p, s) : matmul_blocks<FA, FB, false>(p, s);
 }
 
-hipError_t launch_matmul_blocks(const MatMulBlocksArgs &p, hipStream_t s) {
+hipError_t launch_matmul_blocks(const MatMulBlocksArgs &given, hipStream_t s) {
+    MatMulBlocksArgs p = given;
+    if (const int64_t bytes = matmul_blocks_part_bytes(given)) {
+        const uint32_t row = (uint32_t)((p.k + 15) / 16), total = (uint32_t)(bytes / 16);
+        k_matmul_blocks_rows<<<(total + 255) / 256, 256, 0, s>>>(given, (uint4 *)p.part, make_fastdiv(row), total);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+        p.k = 16 * (int64_t)row;
+        p.a = (const uint8_t *)p.part;
+        p.b = p.a + p.m * p.k;
+    }
     if (p.fmt_a == kFloat8E4M3FN)
         return p.fmt_b == kFloat8E4M3FN ? matmul_blocks<kFloat8E4M3FN, kFloat8E4M3FN>(p, s)
                                         : matmul_blocks<kFloat8E4M3FN, kFloat8E5M2>(p, s);

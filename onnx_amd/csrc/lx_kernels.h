@@ -252,7 +252,9 @@ struct MatMulBlocksArgs {
     float *y;
     int64_t m, n, k;
     int32_t fmt_a, fmt_b, b_rows;
+    void *part;  // matmul_blocks_part_bytes of scratch, 16-byte aligned
 };
+int64_t matmul_blocks_part_bytes(const MatMulBlocksArgs &p);
 hipError_t launch_matmul_blocks(const MatMulBlocksArgs &p, hipStream_t s);
 
 // TokenLogProbs over t rows of v logits (v > 0): the log-probability of ids[row] (Int32 / Int64; null: none), the
