@@ -17,7 +17,7 @@ using System.Linq;
 using static OpResult;
 using CPU = CPUExecutionProvider;
 
-public unsafe class HipExecutionProvider : Runtime
+public unsafe partial class HipExecutionProvider : Runtime
 {
     /// <summary>The operators that run on the device; Node.ExecuteHIP sends the others to CPUExecutionProvider on
     /// host copies.</summary>

@@ -2595,7 +2595,8 @@ extern "C" int lx_QuantizeBlocks(const lx_tensor *X, int64_t to, int64_t block_r
     int64_t mats = 1, rows = 1;
     for (int i = 0; i < X->rank - 1; i++) (block_rows == 1 || i == X->rank - 2 ? rows : mats) *= X->dims[i];
     if (block_rows == 128) sd[X->rank - 2] = blocks128(rows);
-    if (!Q || !scales || Q == scales) return set_err(LX_ERR_INVALID_ARGUMENT, "The output tensor handle is null.");
+    if (!Q || !scales) return set_err(LX_ERR_INVALID_ARGUMENT, "The output tensor handle is null.");
+    if (Q == scales) return set_err(LX_ERR_INVALID_ARGUMENT, "Two outputs share one tensor handle.");
     OutputGuard gq(Q), gs(scales);
     if ((st = prepare_output(Q, (int)to, X->rank, X->dims)) || (st = prepare_output(scales, LX_FLOAT, X->rank, sd))) return st;
     if ((st = check_element_alignment(scales, "scales")) || (st = check_apart(Q, "Q", X, "X")) ||

@@ -184,8 +184,8 @@ template <int FMT> static hipError_t quantize(const QuantizeArgs &a, hipStream_t
     // four values a lane need rows of whole float4s; others go value by value, 32 neighbours at a time
     const bool vec = a.k % 4 == 0 && ((uintptr_t)a.x & 15) == 0 && ((uintptr_t)a.q & 3) == 0;
     if (a.block_rows == 1) {
-        // in row ranges of fewer than 2^31 blocks
-        const int64_t rows = a.mats * a.rows, most = std::max<int64_t>(1, ((int64_t)1 << 30) / kb);
+        // in row ranges of at most 2^28 blocks (a launch takes fewer than 2^32 threads)
+        const int64_t rows = a.mats * a.rows, most = std::max<int64_t>(1, ((int64_t)1 << 28) / kb);
         for (int64_t r = 0; r < rows; r += most) {
             const uint32_t blocks = (uint32_t)(std::min(most, rows - r) * kb);
             const float *x = a.x + r * a.k;

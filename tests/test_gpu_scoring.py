@@ -416,6 +416,59 @@ def test_scoring_head_captured_and_replayed(hip):
             assert torch.equal(a.view(torch.uint8), b.view(torch.uint8)), i
 
 
+def test_product_of_odd_rows_captured_and_replayed(hip):
+    """A product that copies its rows first: the copy lives in the graph's own memory."""
+    rng = np.random.default_rng(2)
+    m, k, n = 1100, 385, 1100
+    (a, sa), (b, sb) = operand(rng, m, k, E4M3, True), operand(rng, n, k, E5M2, False)
+    HIP, wrap = hip.HipExecutionProvider, hip.DeviceTensor.wrap_torch
+    ta = torch.from_numpy(a).cuda().view(torch.float8_e4m3fn)
+    args = [wrap(ta), dev(hip, sa), dev(hip, b, E5M2), dev(hip, sb)]
+    y = torch.empty((m, n), device="cuda")
+    wy = wrap(y)
+    assert HIP.MatMulBlocks(*args, out=wy).Code == 0
+    torch.cuda.synchronize()
+    stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    try:
+        hip.set_stream(stream.cuda_stream)
+        with torch.cuda.graph(graph, stream=stream):
+            assert HIP.MatMulBlocks(*args, out=wy).Code == 0
+    finally:
+        hip.set_stream(None)
+    for i in range(4):
+        c = np.roll(a, i, 0)
+        ta.view(torch.uint8).copy_(torch.from_numpy(c))
+        y.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        replayed = y.cpu().numpy()
+        eager, = ok(HIP.MatMulBlocks(*args))
+        assert np.array_equal(replayed, eager)
+        near(eager, *R.matmul(R.decode(c, E4M3), sa, R.decode(b, E5M2), sb))
+
+
+def test_products_on_another_stream_follow_its_work(hip):
+    """set_stream: operands written on that stream just before, outputs read on it just after."""
+    rng = np.random.default_rng(4)
+    (a, sa), (b, sb) = operand(rng, 70, 512, E4M3, True), operand(rng, 300, 512, E4M3, False)
+    want, err = R.matmul(R.decode(a, E4M3), sa, R.decode(b, E4M3), sb)
+    src, ta = torch.from_numpy(a).cuda(), torch.zeros((70, 512), device="cuda", dtype=torch.uint8)
+    y = torch.empty((70, 300), device="cuda")
+    args = [hip.DeviceTensor.wrap_torch(ta.view(torch.float8_e4m3fn)), dev(hip, sa), dev(hip, b, E4M3), dev(hip, sb)]
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream()
+    try:
+        hip.set_stream(stream.cuda_stream)
+        with torch.cuda.stream(stream):
+            ta.copy_(src)
+            assert hip.HipExecutionProvider.MatMulBlocks(*args, out=hip.DeviceTensor.wrap_torch(y)).Code == 0
+            got = y.cpu().numpy()
+    finally:
+        hip.set_stream(None)
+    near(got, want, err)
+
+
 # ---- refusals ---------------------------------------------------------------------------------------------------
 def refused(r, code, part=""):
     assert r.Status.name == "Failure" and r.Code == code and part in r.Message, (r.Code, r.Message)
@@ -462,6 +515,9 @@ def test_refusals(hip):
     refused(M(a, sa, b, E((2, 3), f32)), L.ERR_WRONG_INPUT_SHAPE, "b_scale")
     refused(M(a, sa, b, sb, bias=E((299,), f32)), L.ERR_WRONG_INPUT_SHAPE, "bias")
     refused(M(a, sa, b, sb, out=E((4, 299), f32)), L.ERR_BUFFER_TOO_SMALL)
+    refused(M(E((1, 1 << 23), E4M3), E((1, 1 << 16), f32), E((1, 1 << 23), E4M3), E((1, 1 << 16), f32)), L.ERR_NOT_SUPPORTED, "2^23")
+    many = E((131072, 1), E4M3), E((131072, 1), f32), E((65568, 1), E4M3), E((513, 1), f32)
+    refused(M(*many), L.ERR_NOT_SUPPORTED, "2^23")
     big = E((4, 300), f32)
     inside = hip.DeviceTensor.wrap(big.h.data + 128, (4, 256), E4M3, 1024, keepalive=big)
     refused(M(inside, sa, b, sb, out=big), L.ERR_INVALID_ARGUMENT, "shares storage")
