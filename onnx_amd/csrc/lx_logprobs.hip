@@ -409,13 +409,17 @@ __global__ __launch_bounds__(kLpBlock) void k_logprobs_join(LogProbsArgs a, int 
 }
 
 // How rows are read, by the time of a call (us, top 5 unless said):
-//   up to 4096 logits a wave each (4096x4000 19 against 33 with a workgroup each);
+//   up to 1024 logits, or from 512 rows on up to 4096, a wave each (4000x1000 9.9 against 25.2 with a workgroup of 256
+//     each, 1000x4000 9.6 against 10.4, but 64x4000 8.7 against 6.8);
 //   up to 24576, or from 384 rows on, a workgroup of 256 each (64x10000 7.9 against 9.3 with 1024 threads and 10.5 in
 //     parts, 384x30522 16.4 against 22.6 and 20.7, 700x131072 75.6 against 85.0 and 89.1);
 //   few rows of more than 32768 in parts, joined by a second launch: about four workgroups a CU over all rows, parts of at
 //     least 2048 logits (1x131072 top 20 11.5 against 22.8 with 1024 threads, 64x50001 13.6 against 14.2);
 //   the others a workgroup of 1024 each (192x65536 16.6 against 23.3 with 256 and 21.0 in parts, 64x30522 11.3, 12.2, 13.1).
-static int lp_team(const LogProbsArgs &a) { return a.v <= 4096 ? 64 : a.v <= 24576 || a.t >= 384 ? 256 : 1024; }
+static int lp_team(const LogProbsArgs &a) {
+    if (a.v <= 1024 || (a.v <= 4096 && a.t >= 512)) return 64;
+    return a.v <= 24576 || a.t >= 384 ? 256 : 1024;
+}
 static int lp_split(const LogProbsArgs &a) {
     if (a.v <= 32768 || a.t >= 96) return 1;
     return (int)std::min<int64_t>({(1024 + a.t - 1) / a.t, a.v / 2048, kLpSplit});
