@@ -77,6 +77,7 @@ __device__ __forceinline__ float f8_finite_abs(float x) {
 }
 
 // Blocks of one row: 32 lanes a block, four values a lane, U blocks at once (their loads and reductions overlap).
+// Bound by memory: [16384, 2048] 33.4 us, 5.0 TB/s, the rate of a large copy (one block at once: 42.7).
 template <int FMT, bool VEC, int U>
 __global__ __launch_bounds__(256) void k_quantize_rows(const float *__restrict__ x, uint8_t *__restrict__ q,
                                                        float *__restrict__ s, int64_t k, FastDiv kb, uint32_t blocks) {
@@ -276,6 +277,9 @@ __device__ __forceinline__ uint4 f8_tail16(uint4 v, int c, int k) {
 // bits in LDS (half the traffic of bf16) and are converted as a wave reads them.  Row r's 16-byte chunk c lies at
 // slot c ^ ((r >> 1) & 7): the 32 rows a fragment read touches then spread over all banks.
 // Operands need rows of whole 16-byte chunks (k a multiple of 16, aligned storage) and tiles within 2^31 bytes.
+// 8192x4096x8192: 474 us, 1.16 PFLOP/s, where the library's bf16 product of 8192^3 reaches 1.25.  The matrix unit is busy
+// in 57% of the cycles; each of its instructions (32 cycles) comes with four conversions and two scalings (24), and
+// under this load the clock falls to 1.6 to 1.9 GHz: fewer cycles no longer mean as much less time.
 __device__ __forceinline__ uint32_t f8_lds(const void *p) {
     return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char *)p;
 }

@@ -13,6 +13,9 @@
 // and the k-th largest over 64 groups of threads bounds the k-th largest logit from below (k distinct units reach
 // it).  Only the logits of threads whose own largest reaches the bound are read again, and only logits that reach it
 // are ranked, by counting; equal logits rank by index.
+//
+// Many rows are bound by memory: [4096, 30522] 91 us, 5.5 TB/s (with the top 5 about 105).  Few rows are bound by
+// launches and the waits of the ranking: [1, 131072] 7 us in two launches, 11.4 with the top 20.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
