@@ -251,7 +251,9 @@ int lx_QuantizeBlocks(const lx_tensor *X, int64_t to, int64_t block_rows, lx_ten
  * A[..., m, k] * B[n, k]), plus bias[n] when bias is not NULL.  A [..., M, K] (or [K]) and B [N, K] are 8-bit
  * codes of either type, each its own; B is stored as [N, K] (a weight matrix by output channel).  a_scale is
  * [..., M, ceil(K / 128)]; b_scale is [ceil(N / 128), ceil(K / 128)] (n' = n / 128) or [N, ceil(K / 128)]
- * (n' = n).  Y is Float; sums are Float, products exact.  A row of A that holds NaN gives a row of NaN. */
+ * (n' = n).  Y is Float; products of codes are exact, sums Float, a block's sum is multiplied by the rounded
+ * a_scale * b_scale (finite ones are expected).  A row of A that holds NaN gives a row of NaN.  K below 2^23, at
+ * most 2^23 tiles of 32 x 32 results (LX_ERR_NOT_SUPPORTED). */
 int lx_MatMulBlocks(const lx_tensor *A, const lx_tensor *a_scale, const lx_tensor *B, const lx_tensor *b_scale,
                     const lx_tensor *bias, lx_tensor *Y);
 /* For each row of logits [..., V] (Float): log_probs [...] = log softmax(logits)[ids], for ids [...] (Int32 or

@@ -783,7 +783,7 @@ int64_t matmul_blocks_part_bytes(const MatMulBlocksArgs &p) {
 }
 
 // The kernel of a product by its tiles of Y, one workgroup each, against the chip's 256 CUs (us on one device, e4m3):
-//   128x128 from 256 of them on: [512,768]x[30522,768] 39 against 48 in tiles of 64x64, 8192x4096x8192 492 against 640;
+//   128x128 from 256 of them on: [512,768]x[30522,768] 39 against 48 in tiles of 64x64, 8192x4096x8192 469 against 640;
 //     4096x768x768, 192 of them, 13.0 against 12.5
 //   64x64 from 257 on: 2048x1024x1024 11.4 against 12.9 with waves over K; 1024x1024x1024, 256 of them, 8.6 against 7.5
 //   64x64 with waves over K from 129 on, and for rows that are not whole chunks: 788x768x768 6.7 against 7.2 in tiles
